@@ -21,13 +21,33 @@ FLAG_KERNEL_STREAM = 2
 FLAG_KERNEL_REGISTER = 4
 FLAG_KERNEL_TENSOR = 8
 FLAG_EPILOGUE_GELU = 16
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 30
+
+
+class PagedKVStruct(ctypes.Structure):
+    """aria_paged_kv."""
+    _fields_ = [("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p), ("page_stride", ctypes.c_longlong),
+                ("slot_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong), ("num_pages", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("dtype", ctypes.c_int), ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int),
+                ("max_pages", ctypes.c_int), ("lens", ctypes.c_void_p)]
+
+
+class LogitRulesStruct(ctypes.Structure):
+    """aria_logit_rules."""
+    _fields_ = [("history", ctypes.c_void_p), ("history_row", ctypes.c_longlong), ("history_cap", ctypes.c_int),
+                ("history_lens", ctypes.c_void_p), ("prompt_lens", ctypes.c_void_p), ("repetition", ctypes.c_void_p),
+                ("frequency", ctypes.c_void_p), ("presence", ctypes.c_void_p), ("bias_tokens", ctypes.c_void_p),
+                ("bias_values", ctypes.c_void_p), ("bias_row", ctypes.c_longlong), ("biases", ctypes.c_int),
+                ("allowed", ctypes.c_void_p), ("allowed_row", ctypes.c_longlong)]
+
 
 # every symbol include/aria_q4.h declares: (restype, argtypes)
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
 _I = ctypes.c_int
 _F = ctypes.c_float
+_L = ctypes.c_longlong
 SIGNATURES = {
     "aria_q4_0_packed_bytes": (_SZ, [_SZ]),
     "aria_q4_0_pack_f16": (_I, [_P, _SZ, _P, _P]),
@@ -50,6 +70,14 @@ SIGNATURES = {
     "aria_attention_decode": (_I, [_P, _I, _I, _I, _P, _P, _I, _P, _P, _P]),
     "aria_flash_attn_fwd": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _F, _P]),
     "aria_attention_prefill": (_I, [_P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P]),
+    "aria_attention_paged_workspace_bytes": (_SZ, [_P, _I, _I, _I]),
+    "aria_attention_paged": (_I, [_P, _I, _I, _P, _L, _L, _P, _P, _L, _L, _F, _P, _L, _L, _P, _P, _P, _L, _P, _P, _P,
+                                  _SZ, _P]),
+    "aria_prompt_weights": (_I, [_P, _L, _L, _L, _P, _L, _L, _L, _I, _I, _I, _I, _I, _I, _P, _F, _I, _P, _L, _L, _P]),
+    "aria_cache_evict_workspace_bytes": (_SZ, [_P, _I, _I]),
+    "aria_cache_evict": (_I, [_P, _I, _P, _P, _P, _P, _L, _P, _I, _I, _I, _P, _P, _SZ, _P]),
+    "aria_logits_workspace_bytes": (_SZ, [_I]),
+    "aria_logits_adjust": (_I, [_P, _P, _I, _L, _I, _I, _P, _I, _L, _P, _P, _SZ, _P]),
     "aria_p2p_alloc": (_I, [_SZ, _P]),
     "aria_p2p_free": (_I, [_P]),
     "aria_p2p_ipc_handle": (_I, [_P, _P]),

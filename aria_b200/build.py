@@ -21,8 +21,9 @@ CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libaria_q4.so")
 SOURCES = ["q4_pack.cu", "q4_gemv.cu", "q4_decode.cu", "q4_gemm_tc.cu", "q4_layer.cu", "attn_prefill.cu",
-           "p2p_allreduce.cu", "q4_capi.cu"]
-HEADERS = ["q4_common.cuh", "q4_tcgen05.cuh"]
+           "attn_paged.cu", "prompt_weights.cu", "cache_evict.cu", "logits.cu", "p2p_allreduce.cu", "q4_capi.cu",
+           "paged_capi.cu"]
+HEADERS = ["q4_common.cuh", "q4_tcgen05.cuh", "q4_status.cuh", "q4_paged.cuh", "q4_logits.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

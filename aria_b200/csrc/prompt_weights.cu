@@ -1,0 +1,416 @@
+// prompt_weights.cu -- the attention weight every position of a prompt has received,
+// on the 5th-generation tensor cores (tcgen05, sm_100a).
+//
+// After the prompt's causal attention (its log-sum-exp rows are kept), for key/value
+// head hk of G query heads and key position s:
+//   w[b][hk][s] = sum over the group's heads h and queries t >= max(s, first) of
+//                 exp(scale q[b][t][h] . k[b][s][hk] - lse[b][h][t])
+// the start of the running sums that eviction ranks positions by.
+//
+// The product is computed transposed, S = K Q^T: a block of 128 keys is the A operand
+// (TMEM lanes = keys) and stays in shared memory while the blocks of 128 queries of
+// every head of the group stream past as B.  A thread then owns one key and adds up
+// its row of S in registers: no reduction across threads, nothing but the finished
+// sums leaves the SM.  Per 128 x 128 block: 2 dh / 128 MMA cycles x 128 (256 at
+// dh = 64) against 16384 exponentials at 16 a cycle (1024 cycles), so the exponential
+// unit is the bound.
+//
+// Persistent, one CTA per SM; an item is (sequence, key/value head, key block), the
+// first blocks (most queries) first.  Twelve warps:
+//   warp 0      TMA producer: K blocks (two buffers), Q blocks into a ring
+//   warp 1      TMEM allocator and single-thread MMA issuer
+//   warps 2-9   sums: two warps per TMEM lane quadrant, one per half of the queries
+//   warp 10     lse rows of the query blocks -> shared memory, in the log2 domain;
+//               +inf for queries before `first` or past the end, whose terms vanish
+// Every wait is bounded (one second for the MMA issuer, two for the others; an abort
+// flag; the code in this unit's g_device_error).
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include "q4_common.cuh"
+#include "q4_tcgen05.cuh"
+
+namespace aria_q4 {
+
+constexpr int kPwThreads = 384;
+constexpr int kPwB = 128;     // keys per item, queries per block
+constexpr int kPwS = 4;       // S buffers (128 TMEM columns each) and lse buffers
+
+struct PromptArgs {
+  int B, T, Hkv, G, first;
+  float scale_log2;
+  const float* lse;           // [B][Hq][T]
+  float* w;                   // element strides w_seq, w_head
+  long long w_seq, w_head;
+  int n_kt;                   // key blocks of a sequence
+  unsigned long long wait_ns;
+};
+
+template <int DH>
+struct PromptSmem {
+  static constexpr int kTile = kPwB * DH * 2;
+  static constexpr int kNQ = DH == 64 ? 6 : 4;              // Q ring stages
+  static constexpr int kKOff = 0;                           // [2]
+  static constexpr int kQOff = 2 * kTile;                   // [kNQ]
+  static constexpr int kLseOff = kQOff + kNQ * kTile;       // [kPwS][128] f32
+  static constexpr int kSumOff = kLseOff + kPwS * kPwB * 4;  // [128] f32: the second half's sums
+  static constexpr int kBarOff = kSumOff + kPwB * 4;
+  static constexpr int kBytes = kBarOff + 512 + 1024;
+};
+
+struct PromptItem {
+  int seq, hk, kt, q0, nq;  // query blocks q0 .. q0 + nq - 1 of each head
+};
+__device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, int t) {
+  const int bh = a.B * a.Hkv;
+  PromptItem r;
+  r.kt = t / bh;
+  r.seq = (t % bh) / a.Hkv;
+  r.hk = t % a.Hkv;
+  r.q0 = max(r.kt, a.first / kPwB);
+  r.nq = a.n_kt - r.q0;
+  return r;
+}
+
+template <int DH, bool BF16>
+__global__ void __launch_bounds__(kPwThreads)
+    prompt_weights_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                          const PromptArgs a) {
+  using L = PromptSmem<DH>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);  // [2]
+  uint64_t* k_empty = k_full + 2;                                     // [2] MMA commit after the item's last block
+  uint64_t* q_full = k_empty + 2;                                     // [kNQ]
+  uint64_t* q_empty = q_full + L::kNQ;                                // [kNQ] MMA commit
+  uint64_t* s_full = q_empty + L::kNQ;                                // [kPwS] MMA commit
+  uint64_t* s_empty = s_full + kPwS;                                  // [kPwS] 8 summing warps
+  uint64_t* l_full = s_empty + kPwS;                                  // [kPwS] lse warp
+  uint64_t* pair_bar = l_full + kPwS;                                 // [4] per quadrant: its 2 summing warps
+  uint64_t* mma_drain = pair_bar + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_drain + 1);
+  int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  float* lse_s = reinterpret_cast<float*>(smem + L::kLseOff);
+  float* half_sum = reinterpret_cast<float*>(smem + L::kSumOff);
+  auto give_up = [&](int wait_result, int code) {
+    if (wait_result == tc::kWaitTimeout) tc::record_error(code);
+    atomicExch(abort_flag, 1);
+  };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_items = a.n_kt * a.B * a.Hkv;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; s++) {
+      tc::mbar_init(&k_full[s], 1);
+      tc::mbar_init(&k_empty[s], 1);
+    }
+    for (int s = 0; s < L::kNQ; s++) {
+      tc::mbar_init(&q_full[s], 1);
+      tc::mbar_init(&q_empty[s], 1);
+    }
+    for (int s = 0; s < kPwS; s++) {
+      tc::mbar_init(&s_full[s], 1);
+      tc::mbar_init(&s_empty[s], 8);
+      tc::mbar_init(&l_full[s], 1);
+    }
+    for (int s = 0; s < 4; s++) tc::mbar_init(&pair_bar[s], 2);
+    tc::mbar_init(mma_drain, 1);
+    *abort_flag = 0;
+    tc::fence_barrier_init();
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(tmem_slot, 512);
+    tc::tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    tc::prefetch_tmap(&tm_q);
+    tc::prefetch_tmap(&tm_k);
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  // Every role walks the same items and query blocks; phases follow the CTA-wide
+  // block counter g and item counter it.
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int g = 0, it = 0;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        const int w = tc::mbar_wait_or_abort(bar, parity, 2 * a.wait_ns, abort_flag);
+        if (w != tc::kWaitOk) {
+          give_up(w, tc::kErrTimeoutEmpty);
+          ok = false;
+        }
+        return ok;
+      };
+      for (int t = blockIdx.x; t < n_items && ok; t += gridDim.x) {
+        const PromptItem im = prompt_item(a, t);
+        if (im.nq <= 0) continue;
+        const int kb = it & 1;
+        if (it >= 2 && !wait(&k_empty[kb], ((it >> 1) - 1) & 1)) break;
+        tc::mbar_arrive_expect_tx(&k_full[kb], L::kTile);
+#pragma unroll
+        for (int c = 0; c < DH / 64; c++)
+          tc::tma_load_4d(smem + L::kKOff + kb * L::kTile + c * (kPwB * 128), &tm_k, 64 * c, im.hk, im.kt * kPwB,
+                          im.seq, &k_full[kb]);
+        it++;
+        for (int h = 0; h < a.G && ok; h++)
+          for (int j = 0; j < im.nq; j++, g++) {
+            const int s = g % L::kNQ, use = g / L::kNQ;
+            if (use >= 1 && !wait(&q_empty[s], (use - 1) & 1)) break;
+            tc::mbar_arrive_expect_tx(&q_full[s], L::kTile);
+#pragma unroll
+            for (int c = 0; c < DH / 64; c++)
+              tc::tma_load_4d(smem + L::kQOff + s * L::kTile + c * (kPwB * 128), &tm_q, 64 * c, im.hk * a.G + h,
+                              (im.q0 + j) * kPwB, im.seq, &q_full[s]);
+          }
+      }
+      // no copy into shared memory may be in flight when the CTA exits
+      for (int i = it > 2 ? it - 2 : 0; i < it; i++) tc::mbar_wait(&k_full[i & 1], (i >> 1) & 1);
+      for (int i = g > L::kNQ ? g - L::kNQ : 0; i < g; i++) tc::mbar_wait(&q_full[i % L::kNQ], (i / L::kNQ) & 1);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc = tc::idesc_f16_f32(128, kPwB) | (BF16 ? (1u << 7) | (1u << 10) : 0u);
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+        const int w = tc::mbar_wait_or_abort(bar, parity, a.wait_ns, abort_flag);
+        if (w != tc::kWaitOk) {
+          give_up(w, code);
+          ok = false;
+        }
+        return ok;
+      };
+      int g = 0, it = 0;
+      for (int t = blockIdx.x; t < n_items && ok; t += gridDim.x) {
+        const PromptItem im = prompt_item(a, t);
+        if (im.nq <= 0) continue;
+        const int kb = it & 1;
+        if (!wait(&k_full[kb], (it >> 1) & 1, tc::kErrTimeoutFull)) break;
+        const uint32_t ks = tc::smem_u32(smem + L::kKOff + kb * L::kTile);
+        const int blocks = a.G * im.nq;
+        for (int j = 0; j < blocks; j++, g++) {
+          const int s = g % L::kNQ, b = g % kPwS;
+          if (!wait(&q_full[s], (g / L::kNQ) & 1, tc::kErrTimeoutFull)) break;
+          if (g >= kPwS && !wait(&s_empty[b], ((g / kPwS) - 1) & 1, tc::kErrTimeoutAccum)) break;
+          tc::tc_fence_after();
+          const uint32_t qs = tc::smem_u32(smem + L::kQOff + s * L::kTile);
+#pragma unroll
+          for (int kk = 0; kk < DH / 16; kk++)
+            tc::umma_f16(tmem_base + (uint32_t)(b * kPwB),
+                         tc::sdesc_k_sw128(ks + (kk >> 2) * (kPwB * 128) + (kk & 3) * 32),
+                         tc::sdesc_k_sw128(qs + (kk >> 2) * (kPwB * 128) + (kk & 3) * 32), idesc, kk > 0 ? 1u : 0u);
+          tc::umma_commit(&s_full[b]);
+          tc::umma_commit(&q_empty[s]);
+          if (j == blocks - 1) tc::umma_commit(&k_empty[kb]);
+        }
+        it++;
+      }
+      if (!ok) {
+        // no MMA of this thread may still write tensor memory when it is freed
+        tc::umma_commit(mma_drain);
+        tc::mbar_wait(mma_drain, 0);
+      }
+    }
+  } else if (warp < 10) {
+    // ------------------------------------------------------------ sums
+    const int qd = warp & 3;           // TMEM lane quadrant
+    const int hf = (warp - 2) >> 2;    // half of the block's queries
+    const int r = qd * 32 + lane;      // key of the block = TMEM lane
+    const uint32_t lane_off = (uint32_t)(qd * 32) << 16;
+    bool ok = true;
+    int pair_uses = 0;
+    auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+      const int w = tc::mbar_wait_or_abort(bar, parity, 2 * a.wait_ns, abort_flag);
+      const bool all_ok = __all_sync(0xffffffffu, w == tc::kWaitOk);
+      const bool any_timeout = __any_sync(0xffffffffu, w == tc::kWaitTimeout);
+      if (!all_ok) {
+        if (lane == 0) give_up(any_timeout ? tc::kWaitTimeout : tc::kWaitAborted, code);
+        ok = false;
+      }
+      return all_ok;
+    };
+    auto pair_sync = [&]() {
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&pair_bar[qd]);
+      const bool met = wait(&pair_bar[qd], (uint32_t)(pair_uses & 1), tc::kErrTimeoutFull);
+      pair_uses++;
+      return met;
+    };
+    int g = 0;
+    for (int t = blockIdx.x; t < n_items && ok; t += gridDim.x) {
+      const PromptItem im = prompt_item(a, t);
+      const int key = im.kt * kPwB + r;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int h = 0; h < a.G && ok; h++)
+        for (int j = 0; j < im.nq; j++, g++) {
+          const int b = g % kPwS;
+          const uint32_t ph = (uint32_t)(g / kPwS) & 1;
+          if (!wait(&l_full[b], ph, tc::kErrTimeoutFull)) break;
+          if (!wait(&s_full[b], ph, tc::kErrTimeoutFull)) break;
+          tc::tc_fence_after();
+          uint32_t sv[64];
+          const uint32_t col = tmem_base + lane_off + (uint32_t)(b * kPwB + hf * 64);
+          tc::tmem_ld_32x32b_x32(col, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
+          tc::tmem_ld_32x32b_x32(col + 32u, *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
+          tc::tmem_ld_wait();
+          tc::reg_tie(sv);
+          const float4* ls = reinterpret_cast<const float4*>(lse_s + b * kPwB + hf * 64);
+          const int q0 = (im.q0 + j) * kPwB + hf * 64;  // this half's first query
+          // queries before the key or before `first` are left out by selection, so
+          // that whatever their rows hold (a NaN too) does not reach the sums
+          const int cmin = max(key, a.first) - q0;
+          if (q0 < max(im.kt * kPwB + kPwB - 1, a.first)) {
+#pragma unroll
+            for (int e = 0; e < 64; e += 4) {
+              const float4 l4 = ls[e >> 2];
+              const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+              for (int u = 0; u < 4; u++) {
+                const float p = tc::ex2_approx(fmaf(__uint_as_float(sv[e + u]), a.scale_log2, -lv[u]));
+                sum[u] += e + u >= cmin ? p : 0.0f;
+              }
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 64; e += 4) {
+              const float4 l4 = ls[e >> 2];
+              const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+              for (int u = 0; u < 4; u++)
+                sum[u] += tc::ex2_approx(fmaf(__uint_as_float(sv[e + u]), a.scale_log2, -lv[u]));
+            }
+          }
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&s_empty[b]);
+        }
+      if (!ok) break;
+      const float mine = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      if (hf == 1) half_sum[r] = mine;
+      if (!pair_sync()) break;
+      if (hf == 0 && key < a.T) a.w[(long long)im.seq * a.w_seq + (long long)im.hk * a.w_head + key] = mine + half_sum[r];
+      if (!pair_sync()) break;  // half_sum may be written again
+    }
+  } else if (warp == 10) {
+    // ------------------------------------------------------------ lse rows
+    int g = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < n_items && ok; t += gridDim.x) {
+      const PromptItem im = prompt_item(a, t);
+      for (int h = 0; h < a.G && ok; h++) {
+        const float* row = a.lse + ((size_t)im.seq * a.Hkv * a.G + im.hk * a.G + h) * a.T;
+        for (int j = 0; j < im.nq; j++, g++) {
+          const int b = g % kPwS;
+          float v[4];
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            const int q = (im.q0 + j) * kPwB + 32 * u + lane;
+            v[u] = q < a.T && q >= a.first ? row[q] * 1.4426950408889634f : INFINITY;
+            if (v[u] == -INFINITY) v[u] = INFINITY;  // a row that saw nothing gives nothing
+          }
+          if (g >= kPwS) {
+            const int w = tc::mbar_wait_or_abort(&s_empty[b], ((g / kPwS) - 1) & 1, 2 * a.wait_ns, abort_flag);
+            if (!__all_sync(0xffffffffu, w == tc::kWaitOk)) {
+              if (lane == 0) give_up(w, tc::kErrTimeoutEmpty);
+              ok = false;
+              break;
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < 4; u++) lse_s[b * kPwB + 32 * u + lane] = v[u];
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(&l_full[b]);
+        }
+      }
+    }
+  }
+
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+typedef CUresult (*PromptEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static PromptEncodeFn prompt_encode_fn() {
+  static PromptEncodeFn fn = []() -> PromptEncodeFn {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    return reinterpret_cast<PromptEncodeFn>(p);
+  }();
+  return fn;
+}
+
+// {DH, H, T, B} view, boxes of 128 positions x 64 columns of one head
+static bool prompt_tmap(CUtensorMap* tm, const void* base, bool bf16, int DH, int H, int T, int B, long long s_head,
+                        long long s_pos, long long s_seq) {
+  PromptEncodeFn enc = prompt_encode_fn();
+  if (!enc) return false;
+  const cuuint64_t dim[4] = {(cuuint64_t)DH, (cuuint64_t)H, (cuuint64_t)T, (cuuint64_t)B};
+  const cuuint64_t str[3] = {(cuuint64_t)s_head * 2, (cuuint64_t)s_pos * 2, (cuuint64_t)s_seq * 2};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)kPwB, 1};
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  return enc(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+             const_cast<void*>(base), dim, str, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DH, bool BF16>
+static cudaError_t launch_prompt_t(const PromptArgs& a, const CUtensorMap& tq, const CUtensorMap& tk,
+                                   cudaStream_t st) {
+  using L = PromptSmem<DH>;
+  auto kern = prompt_weights_kernel<DH, BF16>;
+  int dev = 0, sms = 148;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+  if (e != cudaSuccess) return e;
+  const int items = a.n_kt * a.B * a.Hkv;
+  kern<<<items < sms ? items : sms, kPwThreads, L::kBytes, st>>>(tq, tk, a);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_prompt_weights(const void* q, const void* k, bool bf16, int DH, long long q_seq, long long q_pos,
+                                  long long q_head, long long k_seq, long long k_pos, long long k_head, int B, int T,
+                                  int Hkv, int G, int first, float scale, const float* lse, float* w, long long w_seq,
+                                  long long w_head, cudaStream_t st) {
+  CUtensorMap tq, tk;
+  if (!prompt_tmap(&tq, q, bf16, DH, Hkv * G, T, B, q_head, q_pos, q_seq) ||
+      !prompt_tmap(&tk, k, bf16, DH, Hkv, T, B, k_head, k_pos, k_seq))
+    return cudaErrorInvalidValue;
+  PromptArgs a;
+  a.B = B; a.T = T; a.Hkv = Hkv; a.G = G; a.first = first;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.lse = lse;
+  a.w = w; a.w_seq = w_seq; a.w_head = w_head;
+  a.n_kt = (T + kPwB - 1) / kPwB;
+  a.wait_ns = tc::kWaitLimitNs;
+  if (DH == 64) return bf16 ? launch_prompt_t<64, true>(a, tq, tk, st) : launch_prompt_t<64, false>(a, tq, tk, st);
+  if (DH == 128) return bf16 ? launch_prompt_t<128, true>(a, tq, tk, st) : launch_prompt_t<128, false>(a, tq, tk, st);
+  return cudaErrorInvalidValue;
+}
+
+// Reads and clears this unit's device error flag (synchronous).
+int prompt_take_device_error() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, tc::g_device_error, sizeof(int)) != cudaSuccess) return -1;
+  if (v != 0) cudaMemcpyToSymbol(tc::g_device_error, &zero, sizeof(int));
+  return v;
+}
+
+}  // namespace aria_q4

@@ -1,12 +1,14 @@
 // q4_capi.cu -- extern "C" entry points of libaria_q4.so (declared in
 // include/aria_q4.h).  Argument checking, status codes and kernel selection;
-// the kernels live in q4_pack.cu, q4_gemv.cu, q4_decode.cu and q4_gemm_tc.cu.
+// the kernels live in q4_pack.cu, q4_gemv.cu, q4_decode.cu and q4_gemm_tc.cu (the
+// entry points of the paged cache and of the logits are in paged_capi.cu).
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
 
 #include "../../include/aria_q4.h"
 #include "q4_common.cuh"
+#include "q4_status.cuh"
 
 namespace aria_q4 {
 cudaError_t launch_pack_f16(const uint16_t* src, size_t n, uint8_t* dst, cudaStream_t st);
@@ -32,6 +34,7 @@ size_t tc_workspace_counter_bytes();
 int take_device_error();
 int attn_take_device_error();
 int p2p_take_device_error();
+int prompt_take_device_error();
 cudaError_t launch_p2p_allreduce(const float* const* part, unsigned* const* flag, unsigned* state, int nranks,
                                  int rank, __half* h, int n, unsigned long long wait_ns, cudaStream_t st);
 cudaError_t launch_attention_prefill(const __half* q, const __half* k, const __half* v, int DH, long long s_head,
@@ -73,14 +76,14 @@ using namespace aria_q4;
 
 static thread_local int g_last_cuda_error = 0;
 
-static int cuda_status(cudaError_t e) {
+int aria_q4::cuda_status(cudaError_t e) {
   if (e == cudaSuccess) return ARIA_Q4_OK;
   g_last_cuda_error = (int)e;
   return ARIA_Q4_ECUDA;
 }
 
 // The library is built for sm_100a only; refuse to launch anywhere else.
-static int check_device() {
+int aria_q4::check_device() {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e);
@@ -92,8 +95,6 @@ static int check_device() {
   if (major != 10 || minor != 0) return ARIA_Q4_ENODEVICE;
   return ARIA_Q4_OK;
 }
-
-static bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 static int check_tiled_shape(int layout, int K, int N) {
   if (layout != ARIA_Q4_LAYOUT_KN && layout != ARIA_Q4_LAYOUT_NK) return ARIA_Q4_EINVAL;
@@ -429,7 +430,8 @@ int aria_q4_take_device_error(void) {
   const int a = take_device_error();
   const int b = attn_take_device_error();
   const int c = p2p_take_device_error();
-  return a != 0 ? a : b != 0 ? b : c;
+  const int d = prompt_take_device_error();
+  return a != 0 ? a : b != 0 ? b : c != 0 ? c : d;
 }
 
 // ------------------------------------------------------------------ peer reduction

@@ -1,0 +1,230 @@
+"""A paged, bounded KV cache: attention of one new token over it, the attention
+weight its slots have received, and eviction by that weight (libaria_q4.so).
+
+    kv = PagedKV(k_pages, v_pages, block_table, lens)     # one per layer, kept
+    w  = prompt_weights(q, k, lse)                        # after the prompt's attention
+    out, lse = attention_paged(q, kv, k_new=k, v_new=v, weights=w, slot_pos=p, positions=pos)
+    evict(kv, w, p, next_pos, keep, recent=..., sinks=..., lens_out=...)
+
+The reference's cache (KVCache, lold3344/ARIA src/transformer_cuda.rs:144-155) is
+contiguous and grows with the sequence; paging and eviction have no counterpart
+there.  No fallback: without the library or a B200 every call raises.  Calls run
+on the current stream of the tensors' device; what they write in place, they write
+in the order of that stream.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from ._lib import BF16, F16, PagedKVStruct, call
+
+__all__ = ["PagedKV", "attention_paged", "prompt_weights", "evict"]
+
+_DTYPES = {torch.float16: F16, torch.bfloat16: BF16}
+_WORKSPACES: dict = {}
+
+
+def _stream(dev: torch.device) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _workspace(kind: str, nbytes: int, dev: torch.device, stream: int) -> torch.Tensor:
+    """Zero-filled scratch of one operator on this device and stream, grown on
+    demand; every call leaves it ready for the next."""
+    key = (kind, dev.index, stream)
+    ws = _WORKSPACES.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=dev)
+        _WORKSPACES[key] = ws
+    return ws
+
+
+def _want(t: torch.Tensor, name: str, dtype, shape, dev) -> int:
+    """Pointer of a contiguous tensor of this type, shape and device."""
+    if t.dtype != dtype or t.device != dev or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous {dtype} tensor on {dev}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+class PagedKV:
+    """One layer's cache.  k_pages, v_pages: f16 or bf16 [num_pages][page_size]
+    [kv_heads][head_dim], any strides that are multiples of 8 with contiguous head
+    rows (a transposed view of pages stored head by head is one); block_table: int32
+    [M][max_pages], -1 (or any entry outside the pool) where a sequence has no page;
+    lens: int32 [M], the slots in use.  The tensors are kept and read at every call:
+    write them in place to change pages, table or lengths."""
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor):
+        if not k_pages.is_cuda or k_pages.dim() != 4 or k_pages.dtype not in _DTYPES:
+            raise TypeError("k_pages must be a 4-D f16 or bf16 CUDA tensor")
+        dev = k_pages.device
+        if (v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or v_pages.device != dev
+                or v_pages.stride() != k_pages.stride()):
+            raise ValueError("v_pages must match k_pages in shape, type, device and strides")
+        if k_pages.stride(3) != 1:
+            raise ValueError("the head dimension of the pages must be contiguous")
+        if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.device != dev or (
+                block_table.stride(1) != 1 and block_table.shape[1] > 1):
+            raise TypeError("block_table must be int32 [M][max_pages] on the pages' device, rows contiguous")
+        M = block_table.shape[0]
+        _want(lens, "lens", torch.int32, (M,), dev)
+        n, ps, H, dh = k_pages.shape
+        self.k_pages, self.v_pages, self.block_table, self.lens = k_pages, v_pages, block_table, lens
+        self.M, self.kv_heads, self.head_dim, self.page_size = M, H, dh, ps
+        self.slots = ps * block_table.shape[1]
+        self.dtype, self.device = k_pages.dtype, dev
+        # strides of dimensions of one entry are never used: 8 keeps them valid
+        st = [s if c > 1 else 8 for s, c in zip(k_pages.stride(), k_pages.shape)]
+        self._c = PagedKVStruct(k_pages.data_ptr(), v_pages.data_ptr(), st[0], st[1], st[2], n, ps, H, dh,
+                                _DTYPES[k_pages.dtype], block_table.data_ptr(),
+                                block_table.stride(0) if M > 1 else block_table.shape[1], block_table.shape[1],
+                                lens.data_ptr())
+        self._ref = ctypes.addressof(self._c)
+
+    @classmethod
+    def contiguous(cls, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_heads: int, lens: torch.Tensor,
+                   page_size: int = 16) -> "PagedKV":
+        """A [M][max_seq][d] cache (what attention_prefill fills) as pages in order;
+        max_seq a multiple of page_size."""
+        M, max_seq, d = k_cache.shape
+        if max_seq % page_size or d % kv_heads:
+            raise ValueError("max_seq must be a multiple of page_size and d of kv_heads")
+        per = max_seq // page_size
+        table = torch.arange(M * per, dtype=torch.int32, device=k_cache.device).view(M, per)
+        shape = (M * per, page_size, kv_heads, d // kv_heads)
+        return cls(k_cache.view(shape), v_cache.view(shape), table, lens)
+
+
+def _rows(t: torch.Tensor, name: str, kv: PagedKV, heads: int):
+    """Pointer and (row, head) strides of an [M][heads][head_dim] tensor."""
+    if t.dtype != kv.dtype or t.device != kv.device or t.dim() != 3:
+        raise TypeError(f"{name} must be a 3-D {kv.dtype} tensor on {kv.device}")
+    if t.shape != (kv.M, heads, kv.head_dim):
+        raise ValueError(f"{name} must have shape {(kv.M, heads, kv.head_dim)}, got {tuple(t.shape)}")
+    s = t.stride()
+    if s[2] != 1:
+        raise ValueError(f"the head dimension of {name} must be contiguous")
+    return t.data_ptr(), (s[0] if kv.M > 1 else 8), (s[1] if heads > 1 else 8)
+
+
+def attention_paged(q: torch.Tensor, kv: PagedKV, *, k_new: torch.Tensor | None = None,
+                    v_new: torch.Tensor | None = None, scale: float | None = None, out: torch.Tensor | None = None,
+                    want_lse: bool = False, weights: torch.Tensor | None = None,
+                    weights_out: torch.Tensor | None = None, slot_pos: torch.Tensor | None = None,
+                    positions: torch.Tensor | None = None):
+    """q [M][heads][head_dim] (any strides that are multiples of 8): one new token per
+    sequence.  k_new, v_new [M][kv_heads][head_dim]: its own rows, stored at slot
+    lens[m] and part of the attention (lens is the caller's to advance).  Returns (out
+    [M][heads][head_dim], lse f32 [M][heads] or None); a sequence without slots gives
+    zeros and -inf.  scale defaults to 1 / sqrt(head_dim).
+
+    weights f32 [M][kv_heads][cap >= kv.slots]: the running sums of the attention
+    weight, updated in place or into weights_out; the new token's slot starts from 0,
+    and its entry of slot_pos (int32, the same shape) becomes positions[m]."""
+    heads = q.shape[1] if q.dim() == 3 else 0
+    if heads == 0 or heads % kv.kv_heads:
+        raise ValueError("q must be [M][heads][head_dim] with heads a multiple of kv_heads")
+    qp, q_row, q_head = _rows(q, "q", kv, heads)
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new go together")
+    kp = vp = None
+    n_row = n_head = 0
+    if k_new is not None:
+        kp, n_row, n_head = _rows(k_new, "k_new", kv, kv.kv_heads)
+        vp, v_row, v_head = _rows(v_new, "v_new", kv, kv.kv_heads)
+        if (v_row, v_head) != (n_row, n_head):
+            raise ValueError("k_new and v_new must have the same strides")
+    if out is None:
+        out = torch.empty((kv.M, heads, kv.head_dim), dtype=kv.dtype, device=kv.device)
+    op, o_row, o_head = _rows(out, "out", kv, heads)
+    lse = torch.empty((kv.M, heads), dtype=torch.float32, device=kv.device) if want_lse else None
+    wi = wo = sp = pp = None
+    cap = 0
+    if weights is not None:
+        shape = weights.shape
+        if weights.dim() != 3 or shape[:2] != (kv.M, kv.kv_heads):
+            raise ValueError("weights must be [M][kv_heads][cap]")
+        cap = shape[2]
+        wi = _want(weights, "weights", torch.float32, shape, kv.device)
+        wo = wi if weights_out is None else _want(weights_out, "weights_out", torch.float32, shape, kv.device)
+        if slot_pos is not None:
+            if positions is None or k_new is None:
+                raise ValueError("slot_pos needs positions and k_new")
+            sp = _want(slot_pos, "slot_pos", torch.int32, shape, kv.device)
+            pp = _want(positions, "positions", torch.int32, (kv.M,), kv.device)
+    elif weights_out is not None or slot_pos is not None:
+        raise ValueError("weights_out and slot_pos need weights")
+    lib, stream = _lib.lib(), _stream(kv.device)
+    ws = _workspace("attn", lib.aria_attention_paged_workspace_bytes(kv._ref, kv.M, heads, weights is not None),
+                    kv.device, stream)
+    call("aria_attention_paged", kv._ref, kv.M, heads, qp, q_row, q_head, kp, vp, n_row, n_head,
+         scale if scale is not None else 1.0 / math.sqrt(kv.head_dim), op, o_row, o_head,
+         lse.data_ptr() if lse is not None else None, wi, wo, cap, sp, pp, ws.data_ptr(), ws.numel(), stream)
+    return out, lse
+
+
+def prompt_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, out: torch.Tensor | None = None,
+                   scale: float | None = None, first_query: int = 0) -> torch.Tensor:
+    """The attention weight each position of a prompt received from the queries at
+    positions >= first_query: q [B][T][heads][dh], k [B][T][kv_heads][dh] (strides
+    multiples of 8; views of a packed QKV output serve), lse f32 [B][heads][T] as the
+    prompt's causal attention returned it.  Writes out[:, :, :T] of an f32
+    [B][kv_heads][>= T] tensor with contiguous rows (a new [B][kv_heads][T] one by
+    default) and returns it.  head_dim 64 or 128."""
+    if q.dim() != 4 or k.dim() != 4 or q.dtype not in _DTYPES or k.dtype != q.dtype or not q.is_cuda:
+        raise TypeError("q and k must be 4-D f16 or bf16 CUDA tensors of one type")
+    B, T, heads, dh = q.shape
+    kvh = k.shape[2]
+    if k.shape != (B, T, kvh, dh) or k.device != q.device or kvh == 0 or heads % kvh:
+        raise ValueError("k must be [B][T][kv_heads][dh] with heads a multiple of kv_heads")
+    if (dh > 1 and (q.stride(3) != 1 or k.stride(3) != 1)):
+        raise ValueError("the head dimension of q and k must be contiguous")
+    lp = _want(lse, "lse", torch.float32, (B, heads, T), q.device)
+    if out is None:
+        out = torch.empty((B, kvh, T), dtype=torch.float32, device=q.device)
+    if out.dtype != torch.float32 or out.device != q.device or out.dim() != 3 or out.shape[:2] != (B, kvh) or \
+            out.shape[2] < T or (out.stride(2) != 1 and out.shape[2] > 1):
+        raise ValueError("out must be f32 [B][kv_heads][>= T] with contiguous rows")
+    qs = [s if c > 1 else 8 for s, c in zip(q.stride(), q.shape)]
+    ks = [s if c > 1 else 8 for s, c in zip(k.stride(), k.shape)]
+    call("aria_prompt_weights", q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2],
+         _DTYPES[q.dtype], B, T, heads, kvh, dh, lp, scale if scale is not None else 1.0 / math.sqrt(dh),
+         first_query, out.data_ptr(), out.stride(0), out.stride(1), _stream(q.device))
+    return out
+
+
+def evict(kv: PagedKV, weights: torch.Tensor, slot_pos: torch.Tensor, next_pos: torch.Tensor, keep: int, *,
+          recent: int = 0, sinks: int = 0, weights_out: torch.Tensor | None = None,
+          slot_pos_out: torch.Tensor | None = None, lens_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Cut every row of more than `keep` slots down to `keep`: the positions >= next_pos[m]
+    - recent and < sinks stay, then the largest weights (ties: the lowest slot).  The
+    survivors past `keep` move into the freed slots, in order; weights f32 and slot_pos
+    int32 [M][kv_heads][cap] move with them, in place or into the given outputs, and freed
+    slots end with weight 0 and position -1.  Returns lens_out (int32 [M], another tensor
+    than kv.lens) = min(lens, keep); copy it to kv.lens once every layer that shares kv.lens
+    has been evicted from."""
+    shape = weights.shape
+    if weights.dim() != 3 or shape[:2] != (kv.M, kv.kv_heads):
+        raise ValueError("weights must be [M][kv_heads][cap]")
+    dev = kv.device
+    wi = _want(weights, "weights", torch.float32, shape, dev)
+    pi = _want(slot_pos, "slot_pos", torch.int32, shape, dev)
+    wo = wi if weights_out is None else _want(weights_out, "weights_out", torch.float32, shape, dev)
+    po = pi if slot_pos_out is None else _want(slot_pos_out, "slot_pos_out", torch.int32, shape, dev)
+    npp = _want(next_pos, "next_pos", torch.int32, (kv.M,), dev)
+    if lens_out is None:
+        lens_out = torch.empty_like(kv.lens)
+    lp = _want(lens_out, "lens_out", torch.int32, (kv.M,), dev)
+    if lp == kv.lens.data_ptr() and kv.M > 0:
+        raise ValueError("lens_out must not be kv.lens")
+    lib, stream = _lib.lib(), _stream(dev)
+    ws = _workspace("evict", lib.aria_cache_evict_workspace_bytes(kv._ref, kv.M, keep), dev, stream)
+    call("aria_cache_evict", kv._ref, kv.M, wi, wo, pi, po, shape[2], npp, keep, recent, sinks, lp, ws.data_ptr(),
+         ws.numel(), stream)
+    return lens_out

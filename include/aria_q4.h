@@ -56,7 +56,7 @@ typedef enum {
 
 enum { ARIA_Q4_LAYOUT_KN = 0, ARIA_Q4_LAYOUT_NK = 1 };
 /* element types, numbered like the reference's GGUF dtype ids (:2853, :3213) */
-enum { ARIA_Q4_F32 = 0, ARIA_Q4_F16 = 1 };
+enum { ARIA_Q4_F32 = 0, ARIA_Q4_F16 = 1, ARIA_Q4_BF16 = 30 };
 
 /* ---------------------------------------------------------------- packer */
 
@@ -272,6 +272,118 @@ ARIA_Q4_API int aria_flash_attn_fwd(const uint16_t* q, const uint16_t* k, const 
  * 128; d a multiple of 8; qkv, out and the caches 16-byte aligned. */
 ARIA_Q4_API int aria_attention_prefill(const uint16_t* qkv, int B, int T, int d, int heads, uint16_t* out,
                                        float* lse, uint16_t* k_cache, uint16_t* v_cache, int max_seq, void* stream);
+
+/* ---------------------------------------------------------------- paged, bounded KV cache */
+
+/* Serving many sequences of any length: the KV cache in pages, attention of one
+ * new token over it, the running sum of the attention weight that every slot
+ * receives, and eviction by that sum.  The reference's cache (KVCache,
+ * src/transformer_cuda.rs:144-155) grows without bound and is contiguous; these
+ * have no counterpart there.
+ *
+ * Sequence m's slot j is row j % page_size of page block_table[m][j / page_size];
+ * an entry outside [0, num_pages) has no page, and its slots are absent: not read,
+ * not written, weight 0.  Element strides (multiples of 8) place slot s of page p
+ * of head h at p page_stride + s slot_stride + h head_stride, for K and V alike.
+ * A contiguous cache [M][max_seq][d] is one whose pages lie in order.  head_dim
+ * 32, 64, 128 or 256; pages 16-byte aligned; M <= 4096. */
+typedef struct {
+  void* k_pages;            /* f16 or bf16 (dtype) */
+  void* v_pages;
+  long long page_stride, slot_stride, head_stride;
+  int num_pages, page_size;
+  int kv_heads, head_dim, dtype;
+  const int* block_table;   /* device int [M][table_stride], max_pages used */
+  int table_stride, max_pages;
+  const int* lens;          /* device int [M]: slots in use */
+} aria_paged_kv;
+
+/* Attention of one new token per sequence.  q [M][heads][head_dim] of the cache's
+ * dtype (element strides q_row, q_head); heads a multiple of kv_heads, query head h
+ * reading key/value head h / (heads / kv_heads).  With k_new, v_new ([M][kv_heads]
+ * [head_dim]; both or neither) the new token's rows are stored at slot lens[m] and
+ * take part; lens itself is the caller's to advance.  Over the n slots (lens[m], + 1
+ * with k_new):
+ *     out[m][h] = sum_j p_j v_j,  p_j = exp(scale q.k_j - lse[m][h])
+ * lse [M][heads] (natural log; may be NULL) = ln sum_j exp(scale q.k_j).  A sequence
+ * without slots (n = 0, every page absent, or no room left for the new token) gives
+ * zeros and -inf.  Softmax and sums in f32; p enters the product with V as the sum
+ * of two 16-bit values.
+ * weights_in, weights_out (f32 [M][kv_heads][weights_cap >= max_pages page_size];
+ * both or neither; may be one buffer): for j < n
+ *     weights_out[m][hk][j] = weights_in[m][hk][j] + sum over the group's heads of p_j
+ * where the new token's slot counts from 0; with slot_pos (int, same shape) and
+ * positions (int [M]) that slot's entry becomes positions[m].
+ * workspace: aria_attention_paged_workspace_bytes, 256-byte aligned, zero-filled
+ * before its first use; every call of any shape leaves it ready for the next.
+ * Calls that share one must be ordered. */
+ARIA_Q4_API size_t aria_attention_paged_workspace_bytes(const aria_paged_kv* kv, int M, int heads, int weights);
+ARIA_Q4_API int aria_attention_paged(const aria_paged_kv* kv, int M, int heads, const uint16_t* q, long long q_row,
+                                     long long q_head, const uint16_t* k_new, const uint16_t* v_new,
+                                     long long new_row, long long new_head, float scale, uint16_t* out,
+                                     long long out_row, long long out_head, float* lse, const float* weights_in,
+                                     float* weights_out, long long weights_cap, int* slot_pos, const int* positions,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* The attention weight that every position of a prompt received from the prompt's
+ * queries t >= first_query, given the log-sum-exp rows of its causal attention
+ * (aria_attention_prefill, aria_flash_attn_fwd):
+ *     weights[b][hk][s] = sum over the group's heads h and t >= max(s, first_query)
+ *                         of exp(scale q[b][t][h].k[b][s][hk] - lse[b][h][t])
+ * q, k of dtype with element strides (multiples of 8); lse f32 [B][heads][T]; weights
+ * f32 with strides w_seq, w_head; s = 0 .. T - 1 are written.  A row whose lse is
+ * -inf gives nothing.  head_dim 64 or 128. */
+ARIA_Q4_API int aria_prompt_weights(const uint16_t* q, long long q_seq, long long q_pos, long long q_head,
+                                    const uint16_t* k, long long k_seq, long long k_pos, long long k_head, int dtype,
+                                    int B, int T, int heads, int kv_heads, int head_dim, const float* lse, float scale,
+                                    int first_query, float* weights, long long w_seq, long long w_head, void* stream);
+
+/* Eviction.  Every (sequence, key/value head) row with n = lens[m] > keep slots keeps
+ * those whose position is >= next_pos[m] - recent or < sinks, then those of the
+ * largest weight, ties to the lowest slot (NaN is the lowest weight), `keep` in all.
+ * The i-th survivor at a slot >= keep moves to the i-th slot < keep that is given up
+ * (K and V rows, weight, position); slots keep .. n - 1 end with weight 0 and position
+ * -1, slots past n are not touched.  Rows with n <= keep stay (their weights and
+ * positions are copied when the outputs are other buffers).  lens_out[m] (may be NULL,
+ * must not be lens) = min(n, keep).  recent + sinks <= keep.  Slots without a page
+ * take part with their weights; their rows are not moved. */
+ARIA_Q4_API size_t aria_cache_evict_workspace_bytes(const aria_paged_kv* kv, int M, int keep);
+ARIA_Q4_API int aria_cache_evict(const aria_paged_kv* kv, int M, const float* weights_in, float* weights_out,
+                                 const int* pos_in, int* pos_out, long long cap, const int* next_pos, int keep,
+                                 int recent, int sinks, int* lens_out, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+
+/* ---------------------------------------------------------------- logits */
+
+/* What a row's logits go through before the next token is chosen; NULL members are
+ * left out.  Tokens outside [0, V) in history and bias_tokens are ignored. */
+typedef struct {
+  const int* history;        /* device int [M][history_row]: the tokens so far, oldest first */
+  long long history_row;
+  int history_cap;           /* entries a row can hold */
+  const int* history_lens;   /* [M] */
+  const int* prompt_lens;    /* [M]: entries before it were not generated; NULL: 0 */
+  const float* repetition;   /* [M], 1: none */
+  const float* frequency;    /* [M] */
+  const float* presence;     /* [M] */
+  const int* bias_tokens;    /* [M][bias_row], `biases` used; equal tokens add up in order */
+  const float* bias_values;
+  long long bias_row;
+  int biases;
+  const uint32_t* allowed;   /* [M][allowed_row] (0: one row for all): bit v % 32 of word v / 32 */
+  long long allowed_row;
+} aria_logit_rules;
+
+/* out[m][v], in f32 and in this order: a token of the history has x > 0 ? x / repetition
+ * : x * repetition; one generated c > 0 times loses frequency * c, then presence; biases
+ * are added; -inf where `allowed` has a 0, whatever x was.  logits f32, f16 or bf16; out
+ * of the same type (it may then be the logits) or f32.  token (int [M], may be NULL): the
+ * lowest index of the row's largest f32 result, NaN left out, -1 when none is above -inf;
+ * it needs a workspace (zero-filled before its first use, left so). */
+ARIA_Q4_API size_t aria_logits_workspace_bytes(int M);
+ARIA_Q4_API int aria_logits_adjust(const aria_logit_rules* rules, const void* logits, int dtype, long long logits_row,
+                                   int M, int V, void* out, int out_dtype, long long out_row, int* token,
+                                   void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- multi-GPU */
 
