@@ -17,12 +17,14 @@
 // position, read and written) and 2 x 2 rows per moved slot.
 #include "q4_common.cuh"
 #include "q4_paged.cuh"
+#include "q4_status.cuh"
 
 namespace aria_q4 {
 
 constexpr int kEvictThreads = 512;
 constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kEvictBins = 2048;
+constexpr int kEvictHistBytes = 2 * kEvictBins * (int)sizeof(uint32_t);
 constexpr int kEvictMaxCluster = 8;
 constexpr int kEvictKeys = 40 * 1024;  // keys a CTA can hold in shared memory (160 KB)
 
@@ -278,9 +280,8 @@ size_t evict_workspace_bytes(int M, int Hkv, long long slots, int keep) {
 
 template <bool SMEM_KEYS>
 static cudaError_t launch_evict_t(const EvictArgs& a, size_t smem, cudaStream_t st) {
-  auto kern = cache_evict_kernel<SMEM_KEYS>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
+  constexpr auto kern = cache_evict_kernel<SMEM_KEYS>;
+  if (cudaError_t e = allow_smem<kern>(kEvictHistBytes + kEvictKeys * (int)sizeof(uint32_t))) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.M * a.Hkv * a.cluster));
   cfg.blockDim = dim3(kEvictThreads);
@@ -299,15 +300,13 @@ static cudaError_t launch_evict_t(const EvictArgs& a, size_t smem, cudaStream_t 
 cudaError_t launch_cache_evict(EvictArgs a, void* ws, cudaStream_t st) {
   a.lists = (int*)ws;
   a.list_len = evict_list_len(a.slots, a.keep);
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int sms = sm_count();
   const int rows = a.M * a.Hkv;
   a.cluster = kEvictMaxCluster;
   while (a.cluster > 1 && ((long long)rows * a.cluster > 2 * sms || a.slots / a.cluster < 1024)) a.cluster /= 2;
   const long long share = (a.slots + a.cluster - 1) / a.cluster;
-  const size_t hist = 2 * kEvictBins * sizeof(uint32_t);
-  if (share <= kEvictKeys) return launch_evict_t<true>(a, hist + (size_t)share * sizeof(uint32_t), st);
-  return launch_evict_t<false>(a, hist, st);
+  if (share <= kEvictKeys) return launch_evict_t<true>(a, kEvictHistBytes + (size_t)share * sizeof(uint32_t), st);
+  return launch_evict_t<false>(a, kEvictHistBytes, st);
 }
 
 }  // namespace aria_q4

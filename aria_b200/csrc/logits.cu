@@ -21,6 +21,7 @@
 
 #include "q4_common.cuh"
 #include "q4_logits.cuh"
+#include "q4_status.cuh"
 
 namespace aria_q4 {
 
@@ -186,8 +187,7 @@ static cudaError_t launch_logits_t(const LogitArgs& a, size_t smem, cudaStream_t
 cudaError_t launch_logits_adjust(LogitArgs a, int din, int dout, void* ws, cudaStream_t st) {
   a.best = (unsigned long long*)ws;
   a.arrived = ws ? (unsigned*)(a.best + a.M) : nullptr;
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int sms = sm_count();
   // chunks of 1024 to 8192 tokens: the largest that still gives every SM two
   int chunk = 8192;
   while (chunk > 1024 && (long long)((a.V + chunk - 1) / chunk) * a.M < 2LL * sms) chunk /= 2;

@@ -23,7 +23,6 @@ cudaError_t launch_logits_adjust(LogitArgs a, int din, int dout, void* ws, cudaS
 
 using namespace aria_q4;
 
-static const int kMaxSequences = 4096;           // their tile counts sit in shared memory
 static const long long kMaxSlots = 0x7fffff00;   // of one sequence
 
 static int check_kv(const aria_paged_kv* kv, int M, long long* slots) {
@@ -34,7 +33,7 @@ static int check_kv(const aria_paged_kv* kv, int M, long long* slots) {
   if (kv->dtype != ARIA_Q4_F16 && kv->dtype != ARIA_Q4_BF16) return ARIA_Q4_EINVAL;
   const int dh = kv->head_dim;
   if (dh != 32 && dh != 64 && dh != 128 && dh != 256) return ARIA_Q4_EUNSUPPORTED;
-  if (M > kMaxSequences) return ARIA_Q4_EUNSUPPORTED;
+  if (M > kPagedMaxSequences) return ARIA_Q4_EUNSUPPORTED;
   *slots = (long long)kv->page_size * kv->max_pages;
   if (*slots > kMaxSlots || (long long)M * ((*slots + 15) / 16) > 0x7fffffffLL) return ARIA_Q4_ESIZE;
   if (kv->page_stride % 8 || kv->slot_stride % 8 || kv->head_stride % 8) return ARIA_Q4_EALIGN;
@@ -60,6 +59,8 @@ int aria_attention_paged(const aria_paged_kv* kv, int M, int heads, const uint16
   long long slots = 0;
   if (int s = check_kv(kv, M, &slots)) return s;
   if (heads <= 0 || heads % kv->kv_heads || !(scale == scale)) return ARIA_Q4_EINVAL;
+  // tiles of 16 slots of all pairs (sequence, head), counted in 31 bits
+  if ((long long)M * ((slots + 15) / 16) > 0x7fffffffLL / heads) return ARIA_Q4_ESIZE;
   if ((k_new == nullptr) != (v_new == nullptr) || (weights_in == nullptr) != (weights_out == nullptr))
     return ARIA_Q4_EINVAL;
   if (slot_pos && (!weights_out || !k_new || !positions)) return ARIA_Q4_EINVAL;

@@ -28,6 +28,7 @@
 #include <cuda_bf16.h>
 
 #include "q4_common.cuh"
+#include "q4_status.cuh"
 #include "q4_tcgen05.cuh"
 
 namespace aria_q4 {
@@ -373,13 +374,9 @@ template <int DH, bool BF16>
 static cudaError_t launch_prompt_t(const PromptArgs& a, const CUtensorMap& tq, const CUtensorMap& tk,
                                    cudaStream_t st) {
   using L = PromptSmem<DH>;
-  auto kern = prompt_weights_kernel<DH, BF16>;
-  int dev = 0, sms = 148;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
-  if (e != cudaSuccess) return e;
+  constexpr auto kern = prompt_weights_kernel<DH, BF16>;
+  if (cudaError_t e = allow_smem<kern>(L::kBytes)) return e;
+  const int sms = sm_count();
   const int items = a.n_kt * a.B * a.Hkv;
   kern<<<items < sms ? items : sms, kPwThreads, L::kBytes, st>>>(tq, tk, a);
   return cudaGetLastError();

@@ -82,18 +82,37 @@ int aria_q4::cuda_status(cudaError_t e) {
   return ARIA_Q4_ECUDA;
 }
 
-// The library is built for sm_100a only; refuse to launch anywhere else.
+// The library is built for sm_100a only; refuse to launch anywhere else.  A device's
+// properties do not change while the process lives: asked once, then remembered.
+constexpr int kMaxDevices = 64;
+static int g_device_sms[kMaxDevices];  // multiprocessors of a device that was found fit, else 0
+
 int aria_q4::check_device() {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e);
-  int major = 0, minor = 0;
+  if (dev >= 0 && dev < kMaxDevices && g_device_sms[dev] > 0) return ARIA_Q4_OK;
+  int major = 0, minor = 0, sms = 0;
   e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
   if (e != cudaSuccess) return cuda_status(e);
   e = cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
   if (e != cudaSuccess) return cuda_status(e);
   if (major != 10 || minor != 0) return ARIA_Q4_ENODEVICE;
+  e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return cuda_status(e);
+  if (dev >= 0 && dev < kMaxDevices) g_device_sms[dev] = sms;
   return ARIA_Q4_OK;
+}
+
+int aria_q4::sm_count() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();  // no device: the sizes of one are still answered
+    return sms;
+  }
+  if (dev >= 0 && dev < kMaxDevices && g_device_sms[dev] > 0) return g_device_sms[dev];
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
 }
 
 static int check_tiled_shape(int layout, int K, int N) {

@@ -10,10 +10,12 @@
 
 namespace aria_q4 {
 
-// A pair (sequence, head) of at most this many tiles is not split when every
-// pair has a CTA of its own; otherwise a CTA takes at least kPagedMinShare tiles.
-constexpr int kPagedWholeTiles = 16;
-constexpr int kPagedMinShare = 8;
+constexpr int kPagedMaxSequences = 4096;  // of a call: their lengths and tile counts sit in shared memory
+
+// A pair (sequence, head) of at most this many slots is not split when every
+// pair has a CTA of its own; otherwise a CTA takes at least kPagedMinSlots.
+constexpr int kPagedWholeSlots = 512;
+constexpr int kPagedMinSlots = 128;
 
 struct PagedArgs {
   int M, Hq, Hkv, G;        // sequences, query heads, key/value heads, Hq / Hkv
@@ -26,6 +28,8 @@ struct PagedArgs {
   uint16_t* v_pages_w;
   long long page_stride, slot_stride, head_stride;
   int num_pages, page_size;
+  unsigned page_mul;        // slot / page_size = slot * page_mul >> page_shift
+  int page_shift;
   const int* table;
   int table_stride, max_pages;
   const int* lens;          // slots in use before the call
@@ -37,11 +41,12 @@ struct PagedArgs {
   long long out_row, out_head;
   float* lse;               // [M][Hq], natural log; may be null
   long long slots;          // max_pages * page_size
-  unsigned* counters;       // one per CTA: arrivals at the pair that it begins and others finish
-  float* parts;             // [CTA][2]: states of the pairs that a CTA shares at its start and its end
+  unsigned* counters;       // one per warp: arrivals at the pair that it begins and others finish
+  float* parts;             // [warp][2]: states of the pairs that it shares at its start and at its end
   float* lse2;              // [M][Hq], log2 (accumulated weights only)
   float* scores;            // [M][Hq][score_row], log2 domain
   long long score_row;
+  int stages;               // of every warp's ring
 };
 
 struct EvictArgs {

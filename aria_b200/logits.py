@@ -16,6 +16,7 @@ from .paged import _stream, _want, _workspace
 
 __all__ = ["adjust", "allowed_mask"]
 
+_WS_BYTES: dict = {}
 _DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 
@@ -29,11 +30,20 @@ def allowed_mask(allowed: torch.Tensor) -> torch.Tensor:
     return torch.where(w >= 2**31, w - 2**32, w).to(torch.int32)
 
 
-def _matrix(t: torch.Tensor, name: str, dtype, M: int, dev):
-    if t.dtype != dtype or t.device != dev or t.dim() != 2 or t.shape[0] != M or (
-            t.stride(1) != 1 and t.shape[1] > 1):
-        raise TypeError(f"{name} must be {dtype} [{M}][...] on {dev} with contiguous rows")
-    return t.data_ptr(), t.stride(0) if M > 1 else t.shape[1]
+def _ws_bytes(M: int) -> int:
+    n = _WS_BYTES.get(M)
+    if n is None:
+        n = _WS_BYTES[M] = _lib.lib().aria_logits_workspace_bytes(M)
+    return n
+
+
+def _matrix(t: torch.Tensor, name: str, dtype, M: int, dev: int) -> int:
+    """Row stride of an [M][...] matrix with contiguous rows."""
+    s = t.stride()
+    if t.dtype is not dtype or t.get_device() != dev or len(s) != 2 or t.shape[0] != M or (
+            s[1] != 1 and t.shape[1] > 1):
+        raise TypeError(f"{name} must be {dtype} [{M}][...] on cuda:{dev} with contiguous rows")
+    return s[0] if M > 1 else t.shape[1]
 
 
 def adjust(logits: torch.Tensor, *, out: torch.Tensor | None = None, history: torch.Tensor | None = None,
@@ -55,53 +65,57 @@ def adjust(logits: torch.Tensor, *, out: torch.Tensor | None = None, history: to
     if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in _DTYPES:
         raise TypeError("logits must be an f32, f16 or bf16 [M][V] CUDA tensor")
     M, V = logits.shape
-    dev = logits.device
-    xp, x_row = _matrix(logits, "logits", logits.dtype, M, dev)
+    dev, i32, f32, rows = logits.get_device(), torch.int32, torch.float32, (M,)
+    x_row = _matrix(logits, "logits", logits.dtype, M, dev)
     if out is None:
-        out = torch.empty((M, V), dtype=logits.dtype, device=dev)
-    if out.dtype not in (logits.dtype, torch.float32) or out.shape != logits.shape:
+        out = torch.empty((M, V), dtype=logits.dtype, device=logits.device)
+    if (out.dtype is not logits.dtype and out.dtype is not f32) or out.shape != logits.shape:
         raise TypeError("out must be [M][V] of the logits' type or f32")
-    yp, y_row = _matrix(out, "out", out.dtype, M, dev)
-    r = LogitRulesStruct()
+    y_row = _matrix(out, "out", out.dtype, M, dev)
+    hp = hl = pl = rp = fp = ap = btp = bvp = mp = None
+    h_row = cap = b_row = biases = m_row = 0
     if history is not None:
-        r.history, r.history_row = _matrix(history, "history", torch.int32, M, dev)
-        r.history_cap = history.shape[1]
+        h_row = _matrix(history, "history", i32, M, dev)
         if history_lens is None:
             raise ValueError("history needs history_lens")
-        r.history_lens = _want(history_lens, "history_lens", torch.int32, (M,), dev)
+        hp, cap = history.data_ptr(), history.shape[1]
+        hl = _want(history_lens, "history_lens", i32, rows, dev)
         if prompt_lens is not None:
-            r.prompt_lens = _want(prompt_lens, "prompt_lens", torch.int32, (M,), dev)
+            pl = _want(prompt_lens, "prompt_lens", i32, rows, dev)
     elif repetition is not None or frequency is not None or presence is not None:
         raise ValueError("penalties need a history")
     if repetition is not None:
-        r.repetition = _want(repetition, "repetition", torch.float32, (M,), dev)
+        rp = _want(repetition, "repetition", f32, rows, dev)
     if frequency is not None:
-        r.frequency = _want(frequency, "frequency", torch.float32, (M,), dev)
+        fp = _want(frequency, "frequency", f32, rows, dev)
     if presence is not None:
-        r.presence = _want(presence, "presence", torch.float32, (M,), dev)
-    if (bias_tokens is None) != (bias_values is None):
-        raise ValueError("bias_tokens and bias_values go together")
-    if bias_tokens is not None and bias_tokens.numel() > 0:
-        r.bias_tokens, r.bias_row = _matrix(bias_tokens, "bias_tokens", torch.int32, M, dev)
-        r.bias_values, v_row = _matrix(bias_values, "bias_values", torch.float32, M, dev)
-        if bias_values.shape != bias_tokens.shape or v_row != r.bias_row:
+        ap = _want(presence, "presence", f32, rows, dev)
+    if bias_tokens is not None and bias_values is not None:
+        b_row = _matrix(bias_tokens, "bias_tokens", i32, M, dev)
+        if bias_values.shape != bias_tokens.shape or _matrix(bias_values, "bias_values", f32, M, dev) != b_row:
             raise ValueError("bias_values must match bias_tokens")
-        r.biases = bias_tokens.shape[1]
+        biases = bias_tokens.shape[1]
+        if biases > 0:
+            btp, bvp = bias_tokens.data_ptr(), bias_values.data_ptr()
+    elif bias_tokens is not None or bias_values is not None:
+        raise ValueError("bias_tokens and bias_values go together")
     if allowed is not None:
-        rows = allowed.shape[0] if allowed.dim() == 2 else 0
-        if rows not in (1, M) or allowed.shape[1] != (V + 31) // 32:
+        n = allowed.shape[0] if allowed.dim() == 2 else 0
+        if n not in (1, M) or allowed.shape[1] != (V + 31) // 32:
             raise ValueError("allowed must be int32 [M or 1][ceil(V / 32)]")
-        r.allowed, a_row = _matrix(allowed, "allowed", torch.int32, rows, dev)
-        r.allowed_row = a_row if rows == M else 0
+        m_row = _matrix(allowed, "allowed", i32, n, dev)
+        if n != M:
+            m_row = 0  # one row for all
+        mp = allowed.data_ptr()
+    r = LogitRulesStruct(hp, h_row, cap, hl, pl, rp, fp, ap, btp, bvp, b_row, biases, mp, m_row)
     stream = _stream(dev)
-    tp = wp = None
-    nbytes = 0
+    tp = None
+    ws = (None, 0)
     if want_token or token is not None:
         if token is None:
-            token = torch.empty(M, dtype=torch.int32, device=dev)
-        tp = _want(token, "token", torch.int32, (M,), dev)
-        ws = _workspace("logits", _lib.lib().aria_logits_workspace_bytes(M), dev, stream)
-        wp, nbytes = ws.data_ptr(), ws.numel()
-    call("aria_logits_adjust", ctypes.addressof(r), xp, _DTYPES[logits.dtype], x_row, M, V, yp, _DTYPES[out.dtype],
-         y_row, tp, wp, nbytes, stream)
+            token = torch.empty(rows, dtype=i32, device=logits.device)
+        tp = _want(token, "token", i32, rows, dev)
+        ws = _workspace("logits", _ws_bytes(M), dev, stream)
+    call("aria_logits_adjust", ctypes.addressof(r), logits.data_ptr(), _DTYPES[logits.dtype], x_row, M, V,
+         out.data_ptr(), _DTYPES[out.dtype], y_row, tp, ws[0], ws[1], stream)
     return out, token

@@ -28,25 +28,26 @@ _DTYPES = {torch.float16: F16, torch.bfloat16: BF16}
 _WORKSPACES: dict = {}
 
 
-def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+# The device's current stream as an integer, without building a Stream object: the
+# host's part of a call is a few microseconds in all.
+_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _workspace(kind: str, nbytes: int, dev: torch.device, stream: int) -> torch.Tensor:
-    """Zero-filled scratch of one operator on this device and stream, grown on
-    demand; every call leaves it ready for the next."""
-    key = (kind, dev.index, stream)
+def _workspace(kind: str, nbytes: int, dev: int, stream: int) -> tuple:
+    """(pointer, bytes, tensor) of zero-filled scratch of one operator on this device
+    and stream, grown on demand; every call leaves it ready for the next."""
+    key = (kind, dev, stream)
     ws = _WORKSPACES.get(key)
-    if ws is None or ws.numel() < nbytes:
-        ws = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=dev)
-        _WORKSPACES[key] = ws
+    if ws is None or ws[1] < nbytes:
+        t = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", dev))
+        ws = _WORKSPACES[key] = (t.data_ptr(), t.numel(), t)
     return ws
 
 
-def _want(t: torch.Tensor, name: str, dtype, shape, dev) -> int:
-    """Pointer of a contiguous tensor of this type, shape and device."""
-    if t.dtype != dtype or t.device != dev or not t.is_contiguous():
-        raise TypeError(f"{name} must be a contiguous {dtype} tensor on {dev}")
+def _want(t: torch.Tensor, name: str, dtype, shape, dev: int) -> int:
+    """Pointer of a contiguous tensor of this type and shape on CUDA device `dev`."""
+    if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous {dtype} tensor on cuda:{dev}")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     return t.data_ptr()
@@ -73,12 +74,14 @@ class PagedKV:
                 block_table.stride(1) != 1 and block_table.shape[1] > 1):
             raise TypeError("block_table must be int32 [M][max_pages] on the pages' device, rows contiguous")
         M = block_table.shape[0]
-        _want(lens, "lens", torch.int32, (M,), dev)
+        _want(lens, "lens", torch.int32, (M,), dev.index)
         n, ps, H, dh = k_pages.shape
         self.k_pages, self.v_pages, self.block_table, self.lens = k_pages, v_pages, block_table, lens
         self.M, self.kv_heads, self.head_dim, self.page_size = M, H, dh, ps
         self.slots = ps * block_table.shape[1]
-        self.dtype, self.device = k_pages.dtype, dev
+        self.dtype, self.device, self.index = k_pages.dtype, dev, dev.index
+        self._new_shape = (M, H, dh)
+        self._scale = 1.0 / math.sqrt(dh)
         # strides of dimensions of one entry are never used: 8 keeps them valid
         st = [s if c > 1 else 8 for s, c in zip(k_pages.stride(), k_pages.shape)]
         self._c = PagedKVStruct(k_pages.data_ptr(), v_pages.data_ptr(), st[0], st[1], st[2], n, ps, H, dh,
@@ -86,6 +89,21 @@ class PagedKV:
                                 block_table.stride(0) if M > 1 else block_table.shape[1], block_table.shape[1],
                                 lens.data_ptr())
         self._ref = ctypes.addressof(self._c)
+        self._ws_bytes: dict = {}
+
+    def _workspace_bytes(self, heads: int, weights: bool) -> int:
+        key = (heads, weights)
+        n = self._ws_bytes.get(key)
+        if n is None:
+            n = _lib.lib().aria_attention_paged_workspace_bytes(self._ref, self.M, heads, weights)
+            self._ws_bytes[key] = n
+        return n
+
+    def _evict_bytes(self, keep: int) -> int:
+        n = self._ws_bytes.get(keep)
+        if n is None:
+            n = self._ws_bytes[keep] = _lib.lib().aria_cache_evict_workspace_bytes(self._ref, self.M, keep)
+        return n
 
     @classmethod
     def contiguous(cls, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_heads: int, lens: torch.Tensor,
@@ -101,16 +119,18 @@ class PagedKV:
         return cls(k_cache.view(shape), v_cache.view(shape), table, lens)
 
 
-def _rows(t: torch.Tensor, name: str, kv: PagedKV, heads: int):
-    """Pointer and (row, head) strides of an [M][heads][head_dim] tensor."""
-    if t.dtype != kv.dtype or t.device != kv.device or t.dim() != 3:
-        raise TypeError(f"{name} must be a 3-D {kv.dtype} tensor on {kv.device}")
-    if t.shape != (kv.M, heads, kv.head_dim):
-        raise ValueError(f"{name} must have shape {(kv.M, heads, kv.head_dim)}, got {tuple(t.shape)}")
+def _rows(t: torch.Tensor, name: str, kv: PagedKV, shape) -> tuple:
+    """Strides of a [M][heads][head_dim] tensor with contiguous rows."""
     s = t.stride()
+    if t.dtype is not kv.dtype or t.get_device() != kv.index or len(s) != 3:
+        raise TypeError(f"{name} must be a 3-D {kv.dtype} tensor on cuda:{kv.index}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if s[2] != 1:
         raise ValueError(f"the head dimension of {name} must be contiguous")
-    return t.data_ptr(), (s[0] if kv.M > 1 else 8), (s[1] if heads > 1 else 8)
+    if shape[0] > 1 and shape[1] > 1:
+        return s
+    return (s[0] if shape[0] > 1 else 8, s[1] if shape[1] > 1 else 8, 1)  # strides of one entry are not used
 
 
 def attention_paged(q: torch.Tensor, kv: PagedKV, *, k_new: torch.Tensor | None = None,
@@ -127,45 +147,45 @@ def attention_paged(q: torch.Tensor, kv: PagedKV, *, k_new: torch.Tensor | None 
     weights f32 [M][kv_heads][cap >= kv.slots]: the running sums of the attention
     weight, updated in place or into weights_out; the new token's slot starts from 0,
     and its entry of slot_pos (int32, the same shape) becomes positions[m]."""
-    heads = q.shape[1] if q.dim() == 3 else 0
-    if heads == 0 or heads % kv.kv_heads:
-        raise ValueError("q must be [M][heads][head_dim] with heads a multiple of kv_heads")
-    qp, q_row, q_head = _rows(q, "q", kv, heads)
-    if (k_new is None) != (v_new is None):
-        raise ValueError("k_new and v_new go together")
+    shape = q.shape
+    if len(shape) != 3 or shape[0] != kv.M or shape[2] != kv.head_dim or shape[1] == 0 or shape[1] % kv.kv_heads:
+        raise ValueError(f"q must be [{kv.M}][heads][{kv.head_dim}] with heads a multiple of {kv.kv_heads}")
+    dev, heads = kv.index, shape[1]
+    qs = _rows(q, "q", kv, shape)
     kp = vp = None
-    n_row = n_head = 0
-    if k_new is not None:
-        kp, n_row, n_head = _rows(k_new, "k_new", kv, kv.kv_heads)
-        vp, v_row, v_head = _rows(v_new, "v_new", kv, kv.kv_heads)
-        if (v_row, v_head) != (n_row, n_head):
+    ns = (0, 0)
+    if k_new is not None and v_new is not None:
+        ns = _rows(k_new, "k_new", kv, kv._new_shape)
+        if _rows(v_new, "v_new", kv, kv._new_shape) != ns:
             raise ValueError("k_new and v_new must have the same strides")
+        kp, vp = k_new.data_ptr(), v_new.data_ptr()
+    elif k_new is not None or v_new is not None:
+        raise ValueError("k_new and v_new go together")
     if out is None:
-        out = torch.empty((kv.M, heads, kv.head_dim), dtype=kv.dtype, device=kv.device)
-    op, o_row, o_head = _rows(out, "out", kv, heads)
-    lse = torch.empty((kv.M, heads), dtype=torch.float32, device=kv.device) if want_lse else None
+        out = torch.empty(shape, dtype=kv.dtype, device=kv.device)
+    os_ = _rows(out, "out", kv, shape)
+    lse = torch.empty((shape[0], heads), dtype=torch.float32, device=kv.device) if want_lse else None
     wi = wo = sp = pp = None
     cap = 0
     if weights is not None:
-        shape = weights.shape
-        if weights.dim() != 3 or shape[:2] != (kv.M, kv.kv_heads):
+        wshape = weights.shape
+        if len(wshape) != 3 or wshape[0] != kv.M or wshape[1] != kv.kv_heads:
             raise ValueError("weights must be [M][kv_heads][cap]")
-        cap = shape[2]
-        wi = _want(weights, "weights", torch.float32, shape, kv.device)
-        wo = wi if weights_out is None else _want(weights_out, "weights_out", torch.float32, shape, kv.device)
+        cap = wshape[2]
+        wi = _want(weights, "weights", torch.float32, wshape, dev)
+        wo = wi if weights_out is None else _want(weights_out, "weights_out", torch.float32, wshape, dev)
         if slot_pos is not None:
             if positions is None or k_new is None:
                 raise ValueError("slot_pos needs positions and k_new")
-            sp = _want(slot_pos, "slot_pos", torch.int32, shape, kv.device)
-            pp = _want(positions, "positions", torch.int32, (kv.M,), kv.device)
+            sp = _want(slot_pos, "slot_pos", torch.int32, wshape, dev)
+            pp = _want(positions, "positions", torch.int32, (kv.M,), dev)
     elif weights_out is not None or slot_pos is not None:
         raise ValueError("weights_out and slot_pos need weights")
-    lib, stream = _lib.lib(), _stream(kv.device)
-    ws = _workspace("attn", lib.aria_attention_paged_workspace_bytes(kv._ref, kv.M, heads, weights is not None),
-                    kv.device, stream)
-    call("aria_attention_paged", kv._ref, kv.M, heads, qp, q_row, q_head, kp, vp, n_row, n_head,
-         scale if scale is not None else 1.0 / math.sqrt(kv.head_dim), op, o_row, o_head,
-         lse.data_ptr() if lse is not None else None, wi, wo, cap, sp, pp, ws.data_ptr(), ws.numel(), stream)
+    stream = _stream(dev)
+    ws = _workspace("attn", kv._workspace_bytes(heads, wi is not None), dev, stream)
+    call("aria_attention_paged", kv._ref, kv.M, heads, q.data_ptr(), qs[0], qs[1], kp, vp, ns[0], ns[1],
+         scale if scale is not None else kv._scale, out.data_ptr(), os_[0], os_[1],
+         lse.data_ptr() if lse is not None else None, wi, wo, cap, sp, pp, ws[0], ws[1], stream)
     return out, lse
 
 
@@ -177,25 +197,27 @@ def prompt_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, out: 
     prompt's causal attention returned it.  Writes out[:, :, :T] of an f32
     [B][kv_heads][>= T] tensor with contiguous rows (a new [B][kv_heads][T] one by
     default) and returns it.  head_dim 64 or 128."""
-    if q.dim() != 4 or k.dim() != 4 or q.dtype not in _DTYPES or k.dtype != q.dtype or not q.is_cuda:
+    if q.dim() != 4 or k.dim() != 4 or q.dtype not in _DTYPES or k.dtype is not q.dtype or not q.is_cuda:
         raise TypeError("q and k must be 4-D f16 or bf16 CUDA tensors of one type")
     B, T, heads, dh = q.shape
-    kvh = k.shape[2]
-    if k.shape != (B, T, kvh, dh) or k.device != q.device or kvh == 0 or heads % kvh:
+    kvh, dev = k.shape[2], q.get_device()
+    if k.shape != (B, T, kvh, dh) or k.get_device() != dev or kvh == 0 or heads % kvh:
         raise ValueError("k must be [B][T][kv_heads][dh] with heads a multiple of kv_heads")
-    if (dh > 1 and (q.stride(3) != 1 or k.stride(3) != 1)):
+    qs, ks = q.stride(), k.stride()
+    if qs[3] != 1 or ks[3] != 1:
         raise ValueError("the head dimension of q and k must be contiguous")
-    lp = _want(lse, "lse", torch.float32, (B, heads, T), q.device)
+    if B == 1 or T == 1 or heads == 1 or kvh == 1:  # strides of one entry are not used
+        qs = [s if c > 1 else 8 for s, c in zip(qs, q.shape)]
+        ks = [s if c > 1 else 8 for s, c in zip(ks, k.shape)]
+    lp = _want(lse, "lse", torch.float32, (B, heads, T), dev)
     if out is None:
         out = torch.empty((B, kvh, T), dtype=torch.float32, device=q.device)
-    if out.dtype != torch.float32 or out.device != q.device or out.dim() != 3 or out.shape[:2] != (B, kvh) or \
+    if out.dtype is not torch.float32 or out.get_device() != dev or out.dim() != 3 or out.shape[:2] != (B, kvh) or \
             out.shape[2] < T or (out.stride(2) != 1 and out.shape[2] > 1):
         raise ValueError("out must be f32 [B][kv_heads][>= T] with contiguous rows")
-    qs = [s if c > 1 else 8 for s, c in zip(q.stride(), q.shape)]
-    ks = [s if c > 1 else 8 for s, c in zip(k.stride(), k.shape)]
     call("aria_prompt_weights", q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2],
          _DTYPES[q.dtype], B, T, heads, kvh, dh, lp, scale if scale is not None else 1.0 / math.sqrt(dh),
-         first_query, out.data_ptr(), out.stride(0), out.stride(1), _stream(q.device))
+         first_query, out.data_ptr(), out.stride(0), out.stride(1), _stream(dev))
     return out
 
 
@@ -212,7 +234,7 @@ def evict(kv: PagedKV, weights: torch.Tensor, slot_pos: torch.Tensor, next_pos: 
     shape = weights.shape
     if weights.dim() != 3 or shape[:2] != (kv.M, kv.kv_heads):
         raise ValueError("weights must be [M][kv_heads][cap]")
-    dev = kv.device
+    dev = kv.index
     wi = _want(weights, "weights", torch.float32, shape, dev)
     pi = _want(slot_pos, "slot_pos", torch.int32, shape, dev)
     wo = wi if weights_out is None else _want(weights_out, "weights_out", torch.float32, shape, dev)
@@ -223,8 +245,7 @@ def evict(kv: PagedKV, weights: torch.Tensor, slot_pos: torch.Tensor, next_pos: 
     lp = _want(lens_out, "lens_out", torch.int32, (kv.M,), dev)
     if lp == kv.lens.data_ptr() and kv.M > 0:
         raise ValueError("lens_out must not be kv.lens")
-    lib, stream = _lib.lib(), _stream(dev)
-    ws = _workspace("evict", lib.aria_cache_evict_workspace_bytes(kv._ref, kv.M, keep), dev, stream)
-    call("aria_cache_evict", kv._ref, kv.M, wi, wo, pi, po, shape[2], npp, keep, recent, sinks, lp, ws.data_ptr(),
-         ws.numel(), stream)
+    stream = _stream(dev)
+    ws = _workspace("evict", kv._evict_bytes(keep), dev, stream)
+    call("aria_cache_evict", kv._ref, kv.M, wi, wo, pi, po, shape[2], npp, keep, recent, sinks, lp, ws[0], ws[1], stream)
     return lens_out
