@@ -21,7 +21,7 @@
 
 namespace aria_q4 {
 
-constexpr int kEvictThreads = 512;
+constexpr int kEvictThreads = 256;
 constexpr int kEvictWarps = kEvictThreads / 32;
 constexpr int kEvictBins = 2048;
 constexpr int kEvictHistBytes = 2 * kEvictBins * (int)sizeof(uint32_t);
@@ -78,7 +78,7 @@ __device__ __forceinline__ void block_scan2(uint32_t& x, uint32_t& y, uint32_t& 
 }
 
 template <bool SMEM_KEYS>
-__global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(const EvictArgs a) {
+__global__ void __launch_bounds__(kEvictThreads, 4) cache_evict_kernel(const EvictArgs a) {
   extern __shared__ uint32_t evict_smem[];
   uint32_t* hist = evict_smem;                      // [2][kEvictBins]
   uint32_t* keys = evict_smem + 2 * kEvictBins;     // this CTA's slots
@@ -106,11 +106,11 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(const EvictA
   // (odd: the threads' shared-memory reads then fall into different banks)
   const int share = (n + cs - 1) / cs;
   const int b = min(n, (int)rank * share), e = min(n, b + share);
-  const bool copy = wout != win;
+  const bool copy_w = wout != win, copy_p = pout != pin;
   if (n <= a.keep) {  // nothing to give up (the whole cluster returns)
     for (int i = b + tid; i < e; i += kEvictThreads) {
-      if (copy) wout[i] = win[i];
-      if (pout != pin) pout[i] = pin[i];
+      if (copy_w) wout[i] = win[i];
+      if (copy_p) pout[i] = pin[i];
     }
     return;
   }
@@ -122,8 +122,15 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(const EvictA
   auto key = [&](int i) { return SMEM_KEYS ? keys[i - b] : make_key(i); };
 
   for (int i = tid; i < 2 * kEvictBins; i += kEvictThreads) hist[i] = 0;
-  if (SMEM_KEYS)
-    for (int i = b + tid; i < e; i += kEvictThreads) keys[i - b] = make_key(i);
+  if (SMEM_KEYS || copy_w || copy_p)
+    for (int i = b + tid; i < e; i += kEvictThreads) {
+      // (outputs of their own get what stays where it is here; holes are overwritten below)
+      const int p = pin[i];
+      const float w = win[i];
+      if (SMEM_KEYS) keys[i - b] = p >= newest || p < a.sinks ? 0xffffffffu : evict_key(w);
+      if (copy_w) wout[i] = i < a.keep ? w : 0.0f;
+      if (copy_p) pout[i] = i < a.keep ? p : -1;
+    }
   __syncthreads();
 
   // ---- the keep-th largest key T, and how many slots with exactly T are kept
@@ -139,11 +146,12 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(const EvictA
       if (pass == 0 || (k >> up) == (prefix >> up)) atomicAdd(&h[(k >> shift) & bmask], 1u);
     }
     cluster_sync();
-    // thread t: bins 2047 - 4 t - (0 .. 3), from the largest key down
-    uint32_t cnt[4], sum = 0;
+    // thread t: bins 2047 - BPT t - (0 .. BPT - 1), from the largest key down
+    constexpr int BPT = kEvictBins / kEvictThreads;
+    uint32_t cnt[BPT], sum = 0;
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
-      const int bin = kEvictBins - 1 - 4 * tid - u;
+    for (int u = 0; u < BPT; u++) {
+      const int bin = kEvictBins - 1 - BPT * tid - u;
       cnt[u] = 0;
       for (int r = 0; r < cs; r++) cnt[u] += peer(&h[bin], (uint32_t)r);
       sum += cnt[u];
@@ -151,9 +159,9 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(const EvictA
     uint32_t before = sum, zero = 0, t0, t1;
     block_scan2(before, zero, t0, t1, ws);
 #pragma unroll
-    for (int u = 0; u < 4; u++) {
+    for (int u = 0; u < BPT; u++) {
       if (before < need && before + cnt[u] >= need) {
-        s_bin = (uint32_t)(kEvictBins - 1 - 4 * tid - u);
+        s_bin = (uint32_t)(kEvictBins - 1 - BPT * tid - u);
         s_above = before;
       }
       before += cnt[u];
@@ -207,16 +215,8 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(const EvictA
   for (int i = i0; i < i1; i++) {
     const uint32_t k = key(i);
     const bool kept = k > T || (k == T && tie++ < need);
-    if (i < a.keep) {
-      if (!kept) {
-        to[holes++] = i;
-      } else {
-        if (copy) wout[i] = win[i];
-        if (pout != pin) pout[i] = pin[i];
-      }
-    } else if (kept) {
-      from[movers++] = i;
-    }
+    if (i < a.keep && !kept) to[holes++] = i;
+    if (i >= a.keep && kept) from[movers++] = i;
   }
   cluster_sync();  // the lists are complete, and no key is read any more
 
@@ -261,10 +261,10 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(const EvictA
         *reinterpret_cast<uint4*>(a.v_pages + dst[u]) = vv[u];
       }
   }
-  cluster_sync();  // in place: the moved weights have been read
+  cluster_sync();  // the moved weights have been read; no CTA reads another's memory any more
   for (int i = max(b, a.keep) + tid; i < e; i += kEvictThreads) {
-    wout[i] = 0.0f;
-    pout[i] = -1;
+    if (!copy_w) wout[i] = 0.0f;
+    if (!copy_p) pout[i] = -1;
   }
 }
 

@@ -27,7 +27,6 @@ struct LogitArgs {
   int* token;                 // [M]; may be null
   unsigned long long* best;   // workspace, zero between calls
   unsigned* arrived;
-  int chunk;                  // tokens per CTA (a multiple of 32)
 };
 
 }  // namespace aria_q4
