@@ -41,7 +41,7 @@ constexpr int kPagedThreads = kPagedWarps * 32;
 
 template <int DH, int RB>
 struct PagedCfg {
-  static constexpr int kTile = DH <= 32 ? 32 : 16;  // slots per ring stage
+  static constexpr int kTile = DH <= 64 ? 32 : 16;  // slots per ring stage
   static constexpr int kRows = 8 * RB;              // query heads per pair
   static constexpr int kKBytes = kTile * DH * 2;
   static constexpr int kStageBytes = 2 * kKBytes;   // K, V
@@ -798,12 +798,7 @@ cudaError_t launch_attention_paged(PagedArgs a, int DH, bool bf16, void* ws, con
   const bool weights = wout != nullptr;
   a.chunks = paged_chunks(DH, a.G);
   a.Hv = a.Hkv * a.chunks;
-  // slot / page_size = slot * page_mul >> page_shift, exact for slots below 2^31:
-  // with 2^(l-1) < d <= 2^l, M = ceil(2^(31+l) / d) fits 32 bits and M d - 2^(31+l) < d
-  int l = 0;
-  while ((1LL << l) < a.page_size) l++;
-  a.page_shift = 31 + l;
-  a.page_mul = (unsigned)(((1ULL << a.page_shift) + a.page_size - 1) / a.page_size);
+  page_divisor(a.page_size, a.page_mul, a.page_shift);
   uint8_t* w = (uint8_t*)ws;
   a.counters = (unsigned*)w;
   w += paged_counter_bytes();

@@ -142,7 +142,7 @@ int aria_cache_evict(const aria_paged_kv* kv, int M, const float* weights_in, fl
   long long slots = 0;
   if (int s = check_kv(kv, M, &slots)) return s;
   if (keep <= 0 || recent < 0 || sinks < 0 || (long long)recent + sinks > keep) return ARIA_Q4_EINVAL;
-  if (cap < slots) return ARIA_Q4_ESIZE;
+  if (cap < slots || slots > kEvictMaxSlots) return ARIA_Q4_ESIZE;
   if (M == 0) return ARIA_Q4_OK;
   if (!weights_in || !weights_out || !pos_in || !pos_out || !next_pos) return ARIA_Q4_EINVAL;
   if ((long long)M * kv->kv_heads > 0x7fffffffLL / 8) return ARIA_Q4_ESIZE;
@@ -163,6 +163,7 @@ int aria_cache_evict(const aria_paged_kv* kv, int M, const float* weights_in, fl
   a.page_size = kv->page_size;
   a.table = kv->block_table;
   a.table_stride = kv->table_stride;
+  a.max_pages = kv->max_pages;
   a.lens = kv->lens;
   a.slots = slots;
   a.weights_in = weights_in;

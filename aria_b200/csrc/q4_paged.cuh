@@ -49,14 +49,18 @@ struct PagedArgs {
   int stages;               // of every warp's ring
 };
 
+constexpr long long kEvictMaxSlots = 12 << 20;  // of a sequence: a bit per slot sits in shared memory
+
 struct EvictArgs {
   int M, Hkv;
   uint16_t* k_pages;
   uint16_t* v_pages;
   long long page_stride, slot_stride, head_stride;
   int num_pages, page_size;
+  unsigned page_mul;         // as above
+  int page_shift;
   const int* table;
-  int table_stride;
+  int table_stride, max_pages;
   const int* lens;
   long long slots;           // the table's width in slots
   const float* weights_in;   // [M][Hkv][cap]; the outputs may be the inputs
@@ -69,9 +73,22 @@ struct EvictArgs {
   int keep, recent, sinks;
   int row_bytes;             // of one K row
   int cluster;
+  int bit_words;             // words of a CTA's bits (a multiple of 4)
   int* lists;                // [M * Hkv][2][list_len]: holes, survivors that move
   long long list_len;
+  int* moves;                // [M * Hkv]: entries of a row's lists
+  int fused;                 // the rows are moved by the kernel that chooses them
+  int segment;               // moves per CTA of the kernel that moves them
 };
+
+// slot / page_size = slot * mul >> shift, exact for slots below 2^31: with
+// 2^(l-1) < d <= 2^l, M = ceil(2^(31+l) / d) fits 32 bits and M d - 2^(31+l) < d
+inline void page_divisor(int page_size, unsigned& mul, int& shift) {
+  int l = 0;
+  while ((1LL << l) < page_size) l++;
+  shift = 31 + l;
+  mul = (unsigned)(((1ULL << shift) + page_size - 1) / page_size);
+}
 
 // Slots sequence m attends over: those in use, and the new token's.  A new
 // token without room in the table leaves the sequence with none.

@@ -346,7 +346,7 @@ ARIA_Q4_API int aria_prompt_weights(const uint16_t* q, long long q_seq, long lon
  * -1, slots past n are not touched.  Rows with n <= keep stay (their weights and
  * positions are copied when the outputs are other buffers).  lens_out[m] (may be NULL,
  * must not be lens) = min(n, keep).  recent + sinks <= keep.  Slots without a page
- * take part with their weights; their rows are not moved. */
+ * take part with their weights; their rows are not moved.  Up to 12 * 2^20 slots. */
 ARIA_Q4_API size_t aria_cache_evict_workspace_bytes(const aria_paged_kv* kv, int M, int keep);
 ARIA_Q4_API int aria_cache_evict(const aria_paged_kv* kv, int M, const float* weights_in, float* weights_out,
                                  const int* pos_in, int* pos_out, long long cap, const int* next_pos, int keep,

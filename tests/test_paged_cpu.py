@@ -68,8 +68,8 @@ def test_workspaces(lib):
     assert size(ctypes.byref(_kv()), 3, 5, 0) == 0 and size(None, 3, 4, 0) == 0
     ev = lib.aria_cache_evict_workspace_bytes
     assert ev(ctypes.byref(_kv()), 3, 64) == 0          # nothing can be given up
-    assert ev(ctypes.byref(_kv()), 3, 63) == 3 * 2 * 2 * 4
-    assert ev(ctypes.byref(_kv()), 3, 10) == 3 * 2 * 2 * 10 * 4
+    assert ev(ctypes.byref(_kv()), 3, 63) == 3 * 2 * (2 + 1) * 4
+    assert ev(ctypes.byref(_kv()), 3, 10) == 3 * 2 * (2 * 10 + 1) * 4
     assert lib.aria_logits_workspace_bytes(7) == 7 * 12 and lib.aria_logits_workspace_bytes(0) == 0
 
 
