@@ -13,15 +13,23 @@
 // its row of S in registers: no reduction across threads, nothing but the finished
 // sums leaves the SM.  Per 128 x 128 block: 2 dh / 128 MMA cycles x 128 (256 at
 // dh = 64) against 16384 exponentials at 16 a cycle (1024 cycles), so the exponential
-// unit is the bound.
+// unit is the bound: it is 84% busy at 2 x 8190 x 32 heads of 128 (597 us at the 1.7 GHz
+// that the power limit leaves).  At dh = 64 one pair in eight goes through a polynomial
+// on the multiply-add pipe instead (558 -> 520 us at that size; two pairs: 531); at 128
+// the added instructions lower the clock by more than they save (597 -> 619).
 //
 // Persistent, one CTA per SM; an item is (sequence, key/value head, key block), the
-// first blocks (most queries) first.  Twelve warps:
+// first blocks (most queries) first, dealt out in alternating directions.  Twenty warps:
 //   warp 0      TMA producer: K blocks (two buffers), Q blocks into a ring
 //   warp 1      TMEM allocator and single-thread MMA issuer
-//   warps 2-9   sums: two warps per TMEM lane quadrant, one per half of the queries
-//   warp 10     lse rows of the query blocks -> shared memory, in the log2 domain;
-//               +inf for queries before `first` or past the end, whose terms vanish
+//   warps 2-17  sums: a warp per TMEM lane quadrant and S buffer, so that the four
+//               warps of a sub-partition are at different blocks and keep its
+//               exponential unit busy through one another's waits.  (Four warps per
+//               block, a quarter of the queries each: 55 us at 4 x 2048 x 14 heads;
+//               two warps: 70 us, the unit 40% busy; so: 41 us.)
+//   warp 18     lse rows of the query blocks -> shared memory, negated, in the log2 domain;
+//               -inf for queries before `first` or past the end, whose terms vanish
+//   warp 19     adds an item's four sums per key and stores them
 // Every wait is bounded (one second for the MMA issuer, two for the others; an abort
 // flag; the code in this unit's g_device_error).
 #include <cuda.h>
@@ -33,7 +41,8 @@
 
 namespace aria_q4 {
 
-constexpr int kPwThreads = 384;
+constexpr int kPwSumWarps = 16;
+constexpr int kPwThreads = (4 + kPwSumWarps) * 32;
 constexpr int kPwB = 128;     // keys per item, queries per block
 constexpr int kPwS = 4;       // S buffers (128 TMEM columns each) and lse buffers
 
@@ -54,15 +63,22 @@ struct PromptSmem {
   static constexpr int kKOff = 0;                           // [2]
   static constexpr int kQOff = 2 * kTile;                   // [kNQ]
   static constexpr int kLseOff = kQOff + kNQ * kTile;       // [kPwS][128] f32
-  static constexpr int kSumOff = kLseOff + kPwS * kPwB * 4;  // [128] f32: the second half's sums
-  static constexpr int kBarOff = kSumOff + kPwB * 4;
+  static constexpr int kSumOff = kLseOff + kPwS * kPwB * 4;  // [2 items][kPwS][128] f32: the buffers' sums
+  static constexpr int kBarOff = kSumOff + 2 * kPwS * kPwB * 4;
   static constexpr int kBytes = kBarOff + 512 + 1024;
 };
 
 struct PromptItem {
   int seq, hk, kt, q0, nq;  // query blocks q0 .. q0 + nq - 1 of each head
 };
-__device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, int t) {
+// Item of CTA blockIdx.x in round t / gridDim.x (t = blockIdx.x + round * gridDim.x):
+// odd rounds run backwards, so that no CTA has the longer item of every round.
+__device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, int t, int n_items) {
+  const int g = (int)gridDim.x, round = t / g;
+  if (round & 1) {
+    const int size = min(g, n_items - round * g);  // the last round may be short
+    t = round * g + (size - 1 - t % g);
+  }
   const int bh = a.B * a.Hkv;
   PromptItem r;
   r.kt = t / bh;
@@ -73,8 +89,54 @@ __device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, int t) {
   return r;
 }
 
+// Two f32 values in a register pair, and arithmetic on both in one instruction.
+__device__ __forceinline__ uint64_t pack2(uint32_t x, uint32_t y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(x), "r"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of two values on the multiply-add pipe: x = n + f with n an integer and |f| <= 1/2
+// (n from the low bits of x + 1.5 2^23), a polynomial in f of degree 5 whose coefficients
+// minimise the largest relative error on that interval (Lawson's iteration; 2.3e-7
+// evaluated in f32), and n added to the exponent.  x below -126 gives 2^-126, x above 127
+// gives 2^127, NaN stays NaN.
+__device__ __forceinline__ uint64_t both(float x) { return pack2(__float_as_uint(x), __float_as_uint(x)); }
+__device__ __forceinline__ void exp2_poly2(float& x, float& y) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-126.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(-126.0f));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(127.0f));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(127.0f));
+  const uint64_t v = pack2(__float_as_uint(x), __float_as_uint(y));
+  const uint64_t t = add2(v, both(12582912.0f));
+  const uint64_t f = fma2(add2(t, both(-12582912.0f)), both(-1.0f), v);
+  uint64_t p = fma2(both(1.3276472e-3f), f, both(9.675541e-3f));
+  p = fma2(p, f, both(5.5507131e-2f));
+  p = fma2(p, f, both(2.402212e-1f));
+  p = fma2(p, f, both(6.9314694e-1f));
+  p = fma2(p, f, both(1.0000001f));
+  float p0, p1, t0, t1;
+  unpack2(p, p0, p1);
+  unpack2(t, t0, t1);
+  x = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
+  y = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
+}
+
 template <int DH, bool BF16>
-__global__ void __launch_bounds__(kPwThreads)
+__global__ void __launch_bounds__(kPwThreads, 1)
     prompt_weights_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                           const PromptArgs a) {
   using L = PromptSmem<DH>;
@@ -84,15 +146,16 @@ __global__ void __launch_bounds__(kPwThreads)
   uint64_t* k_empty = k_full + 2;                                     // [2] MMA commit after the item's last block
   uint64_t* q_full = k_empty + 2;                                     // [kNQ]
   uint64_t* q_empty = q_full + L::kNQ;                                // [kNQ] MMA commit
-  uint64_t* s_full = q_empty + L::kNQ;                                // [kPwS] MMA commit
-  uint64_t* s_empty = s_full + kPwS;                                  // [kPwS] 8 summing warps
-  uint64_t* l_full = s_empty + kPwS;                                  // [kPwS] lse warp
-  uint64_t* pair_bar = l_full + kPwS;                                 // [4] per quadrant: its 2 summing warps
-  uint64_t* mma_drain = pair_bar + 4;
+  uint64_t* s_full = q_empty + L::kNQ;                                // [kPwS] MMA commit and lse warp
+  uint64_t* s_empty = s_full + kPwS;                                  // [kPwS] 4 summing warps: S read
+  uint64_t* l_empty = s_empty + kPwS;                                 // [kPwS] 4 summing warps: lse read
+  uint64_t* p_full = l_empty + kPwS;                                  // [2] all summing warps: an item's sums
+  uint64_t* p_empty = p_full + 2;                                     // [2] warp 19
+  uint64_t* mma_drain = p_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_drain + 1);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   float* lse_s = reinterpret_cast<float*>(smem + L::kLseOff);
-  float* half_sum = reinterpret_cast<float*>(smem + L::kSumOff);
+  float* part_sum = reinterpret_cast<float*>(smem + L::kSumOff);
   auto give_up = [&](int wait_result, int code) {
     if (wait_result == tc::kWaitTimeout) tc::record_error(code);
     atomicExch(abort_flag, 1);
@@ -110,11 +173,14 @@ __global__ void __launch_bounds__(kPwThreads)
       tc::mbar_init(&q_empty[s], 1);
     }
     for (int s = 0; s < kPwS; s++) {
-      tc::mbar_init(&s_full[s], 1);
-      tc::mbar_init(&s_empty[s], 8);
-      tc::mbar_init(&l_full[s], 1);
+      tc::mbar_init(&s_full[s], 2);
+      tc::mbar_init(&s_empty[s], 4);
+      tc::mbar_init(&l_empty[s], 4);
     }
-    for (int s = 0; s < 4; s++) tc::mbar_init(&pair_bar[s], 2);
+    for (int s = 0; s < 2; s++) {
+      tc::mbar_init(&p_full[s], kPwSumWarps);
+      tc::mbar_init(&p_empty[s], 1);
+    }
     tc::mbar_init(mma_drain, 1);
     *abort_flag = 0;
     tc::fence_barrier_init();
@@ -148,7 +214,7 @@ __global__ void __launch_bounds__(kPwThreads)
         return ok;
       };
       for (int t = blockIdx.x; t < n_items && ok; t += gridDim.x) {
-        const PromptItem im = prompt_item(a, t);
+        const PromptItem im = prompt_item(a, t, n_items);
         if (im.nq <= 0) continue;
         const int kb = it & 1;
         if (it >= 2 && !wait(&k_empty[kb], ((it >> 1) - 1) & 1)) break;
@@ -188,7 +254,7 @@ __global__ void __launch_bounds__(kPwThreads)
       };
       int g = 0, it = 0;
       for (int t = blockIdx.x; t < n_items && ok; t += gridDim.x) {
-        const PromptItem im = prompt_item(a, t);
+        const PromptItem im = prompt_item(a, t, n_items);
         if (im.nq <= 0) continue;
         const int kb = it & 1;
         if (!wait(&k_full[kb], (it >> 1) & 1, tc::kErrTimeoutFull)) break;
@@ -217,92 +283,130 @@ __global__ void __launch_bounds__(kPwThreads)
         tc::mbar_wait(mma_drain, 0);
       }
     }
-  } else if (warp < 10) {
+  } else if (warp < 2 + kPwSumWarps) {
     // ------------------------------------------------------------ sums
     const int qd = warp & 3;           // TMEM lane quadrant
-    const int hf = (warp - 2) >> 2;    // half of the block's queries
+    const int b = (warp - 2) >> 2;     // S buffer: blocks g = b, b + kPwS, ...
     const int r = qd * 32 + lane;      // key of the block = TMEM lane
-    const uint32_t lane_off = (uint32_t)(qd * 32) << 16;
+    const uint32_t s_col = tmem_base + ((uint32_t)(qd * 32) << 16) + (uint32_t)(b * kPwB);
     bool ok = true;
-    int pair_uses = 0;
     auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
       const int w = tc::mbar_wait_or_abort(bar, parity, 2 * a.wait_ns, abort_flag);
-      const bool all_ok = __all_sync(0xffffffffu, w == tc::kWaitOk);
+      if (__all_sync(0xffffffffu, w == tc::kWaitOk)) return true;
       const bool any_timeout = __any_sync(0xffffffffu, w == tc::kWaitTimeout);
-      if (!all_ok) {
-        if (lane == 0) give_up(any_timeout ? tc::kWaitTimeout : tc::kWaitAborted, code);
-        ok = false;
-      }
-      return all_ok;
+      if (lane == 0) give_up(any_timeout ? tc::kWaitTimeout : tc::kWaitAborted, code);
+      ok = false;
+      return false;
     };
-    auto pair_sync = [&]() {
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&pair_bar[qd]);
-      const bool met = wait(&pair_bar[qd], (uint32_t)(pair_uses & 1), tc::kErrTimeoutFull);
-      pair_uses++;
-      return met;
-    };
-    int g = 0;
-    for (int t = blockIdx.x; t < n_items && ok; t += gridDim.x) {
-      const PromptItem im = prompt_item(a, t);
-      const int key = im.kt * kPwB + r;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int h = 0; h < a.G && ok; h++)
-        for (int j = 0; j < im.nq; j++, g++) {
-          const int b = g % kPwS;
-          const uint32_t ph = (uint32_t)(g / kPwS) & 1;
-          if (!wait(&l_full[b], ph, tc::kErrTimeoutFull)) break;
-          if (!wait(&s_full[b], ph, tc::kErrTimeoutFull)) break;
-          tc::tc_fence_after();
-          uint32_t sv[64];
-          const uint32_t col = tmem_base + lane_off + (uint32_t)(b * kPwB + hf * 64);
-          tc::tmem_ld_32x32b_x32(col, *reinterpret_cast<uint32_t(*)[32]>(&sv[0]));
-          tc::tmem_ld_32x32b_x32(col + 32u, *reinterpret_cast<uint32_t(*)[32]>(&sv[32]));
+    int g0 = 0, it = 0;    // first block and number of the item
+    uint32_t uses = 0;     // blocks of this buffer so far
+    const uint64_t scale2 = pack2(__float_as_uint(a.scale_log2), __float_as_uint(a.scale_log2));
+    for (int t = blockIdx.x; t < n_items && ok; t += gridDim.x, it++) {
+      const PromptItem im = prompt_item(a, t, n_items);
+      const int key = im.kt * kPwB + r, blocks = im.nq > 0 ? a.G * im.nq : 0;
+      const int masked = max(im.kt * kPwB + kPwB - 1, a.first);  // from this query on nothing is left out
+      uint64_t sum[2] = {0, 0};  // four running sums
+      for (int j = (b - g0) & (kPwS - 1); j < blocks; j += kPwS, uses++) {
+        if (!wait(&s_full[b], uses & 1, tc::kErrTimeoutFull)) break;
+        tc::tc_fence_after();
+        const int q0 = (im.q0 + j % im.nq) * kPwB;
+        uint32_t sv[2][16];
+        tc::tmem_ld_32x32b_x16(s_col, sv[0]);
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
           tc::tmem_ld_wait();
-          tc::reg_tie(sv);
-          const float4* ls = reinterpret_cast<const float4*>(lse_s + b * kPwB + hf * 64);
-          const int q0 = (im.q0 + j) * kPwB + hf * 64;  // this half's first query
-          // queries before the key or before `first` are left out by selection, so
-          // that whatever their rows hold (a NaN too) does not reach the sums
-          const int cmin = max(key, a.first) - q0;
-          if (q0 < max(im.kt * kPwB + kPwB - 1, a.first)) {
+          tc::reg_tie(sv[c & 1]);
+          if (c < 7) {
+            tc::tmem_ld_32x32b_x16(s_col + 16 * (c + 1), sv[(c + 1) & 1]);
+          } else {  // the scores are in registers: the next product may begin
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&s_empty[b]);
+          }
+          const ulonglong2* ls = reinterpret_cast<const ulonglong2*>(lse_s + b * kPwB + c * 16);
+          const int qc = q0 + c * 16;
+          if (qc < masked) {
+            // queries before the key or before `first` are left out by selection, so that
+            // whatever their rows hold (a NaN too) does not reach the sums
+            const int cmin = max(key, a.first) - qc;
 #pragma unroll
-            for (int e = 0; e < 64; e += 4) {
-              const float4 l4 = ls[e >> 2];
-              const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
-#pragma unroll
-              for (int u = 0; u < 4; u++) {
-                const float p = tc::ex2_approx(fmaf(__uint_as_float(sv[e + u]), a.scale_log2, -lv[u]));
-                sum[u] += e + u >= cmin ? p : 0.0f;
-              }
+            for (int e = 0; e < 16; e += 4) {
+              const ulonglong2 l4 = ls[e >> 2];  // -lse of four queries
+              const uint32_t* s4 = &sv[c & 1][e];
+              float p0, p1, p2, p3;
+              unpack2(fma2(pack2(s4[0], s4[1]), scale2, l4.x), p0, p1);
+              unpack2(fma2(pack2(s4[2], s4[3]), scale2, l4.y), p2, p3);
+              p0 = tc::ex2_approx(p0);
+              p1 = tc::ex2_approx(p1);
+              p2 = tc::ex2_approx(p2);
+              p3 = tc::ex2_approx(p3);
+              p0 = e >= cmin ? p0 : 0.0f;
+              p1 = e + 1 >= cmin ? p1 : 0.0f;
+              p2 = e + 2 >= cmin ? p2 : 0.0f;
+              p3 = e + 3 >= cmin ? p3 : 0.0f;
+              sum[0] = add2(sum[0], pack2(__float_as_uint(p0), __float_as_uint(p1)));
+              sum[1] = add2(sum[1], pack2(__float_as_uint(p2), __float_as_uint(p3)));
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < 64; e += 4) {
-              const float4 l4 = ls[e >> 2];
-              const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
-#pragma unroll
-              for (int u = 0; u < 4; u++)
-                sum[u] += tc::ex2_approx(fmaf(__uint_as_float(sv[e + u]), a.scale_log2, -lv[u]));
+            for (int e = 0; e < 16; e += 4) {
+              const ulonglong2 l4 = ls[e >> 2];  // -lse of four queries
+              const uint32_t* s4 = &sv[c & 1][e];
+              float p0, p1, p2, p3;
+              unpack2(fma2(pack2(s4[0], s4[1]), scale2, l4.x), p0, p1);
+              unpack2(fma2(pack2(s4[2], s4[3]), scale2, l4.y), p2, p3);
+              p0 = tc::ex2_approx(p0);
+              p1 = tc::ex2_approx(p1);
+              if (DH == 64 && e == 0) {
+                exp2_poly2(p2, p3);
+              } else {
+                p2 = tc::ex2_approx(p2);
+                p3 = tc::ex2_approx(p3);
+              }
+              sum[0] = add2(sum[0], pack2(__float_as_uint(p0), __float_as_uint(p1)));
+              sum[1] = add2(sum[1], pack2(__float_as_uint(p2), __float_as_uint(p3)));
             }
           }
-          tc::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&s_empty[b]);
         }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&l_empty[b]);
+      }
       if (!ok) break;
-      const float mine = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      if (hf == 1) half_sum[r] = mine;
-      if (!pair_sync()) break;
-      if (hf == 0 && key < a.T) a.w[(long long)im.seq * a.w_seq + (long long)im.hk * a.w_head + key] = mine + half_sum[r];
-      if (!pair_sync()) break;  // half_sum may be written again
+      g0 += blocks;
+      if (it >= 2 && !wait(&p_empty[it & 1], ((it >> 1) - 1) & 1, tc::kErrTimeoutEmpty)) break;
+      float s0, s1, s2, s3;
+      unpack2(sum[0], s0, s1);
+      unpack2(sum[1], s2, s3);
+      part_sum[((it & 1) * kPwS + b) * kPwB + r] = (s0 + s1) + (s2 + s3);
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&p_full[it & 1]);
     }
-  } else if (warp == 10) {
+  } else if (warp == 3 + kPwSumWarps) {
+    // ------------------------------------------------------------ an item's sums -> output
+    int it = 0;
+    for (int t = blockIdx.x; t < n_items; t += gridDim.x, it++) {
+      const PromptItem im = prompt_item(a, t, n_items);
+      const int w = tc::mbar_wait_or_abort(&p_full[it & 1], (it >> 1) & 1, 2 * a.wait_ns, abort_flag);
+      if (!__all_sync(0xffffffffu, w == tc::kWaitOk)) {
+        if (lane == 0) give_up(w, tc::kErrTimeoutFull);
+        break;
+      }
+      const float* ps = part_sum + (it & 1) * kPwS * kPwB;
+#pragma unroll
+      for (int u = 0; u < kPwB / 32; u++) {
+        const int r = 32 * u + lane, key = im.kt * kPwB + r;
+        const float sum = (ps[r] + ps[kPwB + r]) + (ps[2 * kPwB + r] + ps[3 * kPwB + r]);
+        if (key < a.T) a.w[(long long)im.seq * a.w_seq + (long long)im.hk * a.w_head + key] = sum;
+      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&p_empty[it & 1]);
+    }
+  } else if (warp == 2 + kPwSumWarps) {
     // ------------------------------------------------------------ lse rows
     int g = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < n_items && ok; t += gridDim.x) {
-      const PromptItem im = prompt_item(a, t);
+      const PromptItem im = prompt_item(a, t, n_items);
       for (int h = 0; h < a.G && ok; h++) {
         const float* row = a.lse + ((size_t)im.seq * a.Hkv * a.G + im.hk * a.G + h) * a.T;
         for (int j = 0; j < im.nq; j++, g++) {
@@ -311,11 +415,11 @@ __global__ void __launch_bounds__(kPwThreads)
 #pragma unroll
           for (int u = 0; u < 4; u++) {
             const int q = (im.q0 + j) * kPwB + 32 * u + lane;
-            v[u] = q < a.T && q >= a.first ? row[q] * 1.4426950408889634f : INFINITY;
-            if (v[u] == -INFINITY) v[u] = INFINITY;  // a row that saw nothing gives nothing
+            v[u] = q < a.T && q >= a.first ? row[q] * -1.4426950408889634f : -INFINITY;
+            if (v[u] == INFINITY) v[u] = -INFINITY;  // a row that saw nothing gives nothing
           }
           if (g >= kPwS) {
-            const int w = tc::mbar_wait_or_abort(&s_empty[b], ((g / kPwS) - 1) & 1, 2 * a.wait_ns, abort_flag);
+            const int w = tc::mbar_wait_or_abort(&l_empty[b], ((g / kPwS) - 1) & 1, 2 * a.wait_ns, abort_flag);
             if (!__all_sync(0xffffffffu, w == tc::kWaitOk)) {
               if (lane == 0) give_up(w, tc::kErrTimeoutEmpty);
               ok = false;
@@ -325,7 +429,7 @@ __global__ void __launch_bounds__(kPwThreads)
 #pragma unroll
           for (int u = 0; u < 4; u++) lse_s[b * kPwB + 32 * u + lane] = v[u];
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&l_full[b]);
+          if (lane == 0) tc::mbar_arrive(&s_full[b]);
         }
       }
     }
