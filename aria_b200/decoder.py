@@ -142,6 +142,13 @@ class Decoder:
         call("aria_layernorm_f32", self.h.data_ptr(), self.M, self.cfg.d_model, g.data_ptr(), b.data_ptr(),
              LN_EPS, self.xn.data_ptr(), self.cfg.d_model, _stream())
 
+    def _attend(self, i: int) -> None:
+        """Layer i's attention of the new tokens: self.qkv -> self.att, their keys and
+        values into the caches."""
+        call("aria_attention_decode", self.qkv.data_ptr(), self.M, self.cfg.d_model, self.cfg.num_heads,
+             self.k_cache[i].data_ptr(), self.v_cache[i].data_ptr(), self.w.max_seq, self.positions.data_ptr(),
+             self.att.data_ptr(), _stream())
+
     def run(self) -> torch.Tensor:
         """One decode step for the tokens and positions already in
         self.tokens / self.positions (device int32 [M]); returns self.logits."""
@@ -156,9 +163,7 @@ class Decoder:
             else:
                 self._layernorm(p.ln1_g, p.ln1_b)
                 matmul(self.xn, p.qkv, self.qkv, bias=p.b_qkv, const_weights=True)
-            call("aria_attention_decode", self.qkv.data_ptr(), self.M, d, cfg.num_heads,
-                 self.k_cache[i].data_ptr(), self.v_cache[i].data_ptr(), w.max_seq, self.positions.data_ptr(),
-                 self.att.data_ptr(), _stream())
+            self._attend(i)
             matmul(self.att, p.out, self.h, bias=p.b_out, beta=1.0, const_weights=True)
             if fused_ln:
                 matmul_ln(self.h, p.ln2_g, p.ln2_b, p.up, self.u, eps=LN_EPS, bias=p.b_up, activation="gelu",
@@ -202,7 +207,7 @@ class Decoder:
         self._pbuf = buf
         return buf
 
-    def run_prefill(self, T: int, fill_cache: bool = True) -> torch.Tensor:
+    def run_prefill(self, T: int, fill_cache: bool = True, after_attention=None) -> torch.Tensor:
         """The reference's whole-prompt forward (forward_gpu,
         src/transformer_cuda.rs:1518-1873) for the M sequences of T tokens
         already in the prefill token buffer (`prefill` fills it): embedding +
@@ -212,7 +217,8 @@ class Decoder:
         LayerNorm and the LM head over every token (f16 logits [M*T][vocab]).
         With fill_cache, each layer's attention launch also stores its k and v
         rows into the KV caches at positions 0..T-1, so `step` continues at
-        position T."""
+        position T.  after_attention(i, qkv, lse), if given, is called after each
+        layer's attention with its QKV rows and log-sum-exp rows."""
         from .attention import attention_prefill
         cfg, w, b = self.cfg, self.w, self._prefill_buffers(T)
         d, n = cfg.d_model, self.M * T
@@ -229,9 +235,12 @@ class Decoder:
             ln(p.ln1_g, p.ln1_b)
             matmul(b["xn"], p.qkv, b["qkv"], bias=p.b_qkv, const_weights=True)
             # the attention launch also stores this layer's k, v rows into the caches
-            attention_prefill(b["qkv"], self.M, T, cfg.num_heads, out=b["att"],
-                              k_cache=self.k_cache[i] if fill_cache else None,
-                              v_cache=self.v_cache[i] if fill_cache else None)
+            _, lse = attention_prefill(b["qkv"], self.M, T, cfg.num_heads, out=b["att"],
+                                       want_lse=after_attention is not None,
+                                       k_cache=self.k_cache[i] if fill_cache else None,
+                                       v_cache=self.v_cache[i] if fill_cache else None)
+            if after_attention is not None:
+                after_attention(i, b["qkv"], lse)
             matmul(b["att"], p.out, b["h"], bias=p.b_out, beta=1.0, const_weights=True)
             ln(p.ln2_g, p.ln2_b)
             matmul(b["xn"], p.up, b["u"], bias=p.b_up, activation="gelu", const_weights=True)

@@ -1,0 +1,152 @@
+"""Generation with a bounded cache: the decoder of aria_b200/decoder.py over a paged
+KV cache that keeps the `budget` slots of each head with the largest accumulated
+attention weight (and the newest and first positions), its logits adjusted and the next
+token chosen on the GPU.
+
+    dec = BoundedDecoder(DecoderWeights(EfkolosConfig()), M=2, budget=256)
+    tokens = dec.generate(prompts, 100, repetition=1.2)
+
+Per prompt and layer: the prompt's attention fills the cache and returns its log-sum-exp
+rows, `prompt_weights` adds up what every position received, `evict` cuts the cache to the
+budget.  Per token and layer: `attention_paged` stores the new rows, attends and adds to
+the weights; per token: `logits.adjust`; and once a row has outgrown the budget by `slack`
+slots, `evict` again.  No call waits for the GPU.
+
+    python -m aria_b200.generate --prompt 400 --tokens 200 --budget 128
+"""
+from __future__ import annotations
+
+import argparse
+
+import torch
+
+from .decoder import Decoder, DecoderWeights
+from .logits import adjust
+from .paged import PagedKV, attention_paged, evict, prompt_weights
+
+__all__ = ["BoundedDecoder"]
+
+
+class BoundedDecoder(Decoder):
+    """A Decoder whose caches (weights.max_seq slots per sequence, in pages) never hold
+    more than budget + slack slots of a sequence after its prompt.  recent, sinks: the
+    newest and first positions that are always kept."""
+
+    def __init__(self, weights: DecoderWeights, M: int = 1, *, budget: int = 256, recent: int = 32, sinks: int = 4,
+                 slack: int = 16, page_size: int = 16, device="cuda"):
+        super().__init__(weights, M, device)
+        cfg, cap = self.cfg, weights.max_seq
+        if not 0 < budget <= budget + slack < cap or recent + sinks > budget:
+            raise ValueError(f"needs recent + sinks <= budget and budget + slack < max_seq = {cap}")
+        self.budget, self.recent, self.sinks, self.slack = budget, recent, sinks, slack
+        self.lens = torch.zeros(M, dtype=torch.int32, device=device)
+        self._lens_next = torch.zeros_like(self.lens)
+        self.kv = [PagedKV.contiguous(k, v, cfg.num_heads, self.lens, page_size)
+                   for k, v in zip(self.k_cache, self.v_cache)]
+        shape = (M, cfg.num_heads, cap)
+        self.weights = [torch.zeros(shape, dtype=torch.float32, device=device) for _ in self.kv]
+        self.slot_pos = [torch.zeros(shape, dtype=torch.int32, device=device) for _ in self.kv]
+        self._prompt_pos = torch.arange(cap, dtype=torch.int32, device=device).expand(shape)
+        self.used = 0  # slots in use, the same for every sequence
+
+    def _attend(self, i: int) -> None:
+        M, H, dh = self.M, self.cfg.num_heads, self.cfg.head_dim
+        x = self.qkv.view(M, 3, H, dh)
+        attention_paged(x[:, 0], self.kv[i], k_new=x[:, 1], v_new=x[:, 2], out=self.att.view(M, H, dh),
+                        weights=self.weights[i], slot_pos=self.slot_pos[i], positions=self.positions)
+
+    def _evict(self) -> None:
+        """Every layer's rows down to the budget (they share one length)."""
+        if self.used <= self.budget:
+            return
+        for i, kv in enumerate(self.kv):
+            evict(kv, self.weights[i], self.slot_pos[i], self.positions, self.budget, recent=self.recent,
+                  sinks=self.sinks, lens_out=self._lens_next)
+        self.lens.copy_(self._lens_next)
+        self.used = self.budget
+
+    def prefill(self, tokens, fill_cache: bool = True) -> torch.Tensor:
+        """The whole prompts [M][T]; afterwards the caches hold at most `budget` slots and
+        self.positions the position of the next token."""
+        if not fill_cache:
+            return super().prefill(tokens, False)
+        tok = torch.as_tensor(tokens, dtype=torch.int32)
+        if tok.dim() != 2 or tok.shape[0] != self.M:
+            raise ValueError(f"tokens must be [{self.M}][T]")
+        T, (M, H, dh) = tok.shape[1], (self.M, self.cfg.num_heads, self.cfg.head_dim)
+
+        def count(i, qkv, lse):
+            x = qkv.view(M, T, 3, H, dh)
+            prompt_weights(x[:, :, 0], x[:, :, 1], lse, out=self.weights[i])
+            self.slot_pos[i].copy_(self._prompt_pos)
+
+        self._prefill_buffers(T)["tok"].copy_(tok.reshape(-1))
+        logits = self.run_prefill(T, True, after_attention=count)
+        self.positions.fill_(T)
+        self.lens.fill_(T)
+        self.used = T
+        self._evict()
+        return logits
+
+    def advance(self) -> torch.Tensor:
+        """One step for self.tokens at self.positions; returns the f32 logits [M][vocab]."""
+        logits = self.run()
+        self.positions.add_(1)
+        self.lens.add_(1)
+        self.used += 1
+        if self.used >= self.budget + self.slack:
+            self._evict()
+        return logits
+
+    def generate(self, prompts, steps: int, *, repetition: float = 1.0, frequency: float = 0.0, presence: float = 0.0,
+                 bias_tokens: torch.Tensor | None = None, bias_values: torch.Tensor | None = None,
+                 allowed: torch.Tensor | None = None) -> torch.Tensor:
+        """Greedy tokens [M][steps] (int32, on the device) after prompts [M][T]; the
+        penalties count the prompt (repetition) and what was generated (all three), biases
+        and the mask are those of logits.adjust."""
+        prompts = torch.as_tensor(prompts, dtype=torch.int32)
+        M, T = self.M, prompts.shape[1]
+        dev = self.h.device
+        history = torch.zeros(M, T + steps, dtype=torch.int32, device=dev)
+        logits = self.prefill(prompts).view(M, T, -1)[:, -1].float().contiguous()
+        history[:, :T] = prompts.to(dev)
+        n, n_prompt = (torch.full((M,), T, dtype=torch.int32, device=dev) for _ in range(2))
+        params = {k: torch.full((M,), v, dtype=torch.float32, device=dev)
+                  for k, v in (("repetition", repetition), ("frequency", frequency), ("presence", presence))}
+        for s in range(steps):
+            adjust(logits, out=logits, history=history, history_lens=n, prompt_lens=n_prompt, bias_tokens=bias_tokens,
+                   bias_values=bias_values, allowed=allowed, token=self.tokens, **params)
+            history[:, T + s] = self.tokens
+            n.add_(1)
+            if s + 1 < steps:
+                logits = self.advance()
+        return history[:, T:]
+
+
+def main() -> None:
+    from .efkolos import EfkolosConfig
+    ap = argparse.ArgumentParser(description=__doc__.split("\n\n")[0])
+    ap.add_argument("--sequences", type=int, default=2)
+    ap.add_argument("--prompt", type=int, default=400)
+    ap.add_argument("--tokens", type=int, default=200)
+    ap.add_argument("--budget", type=int, default=128)
+    ap.add_argument("--layers", type=int, default=20)
+    a = ap.parse_args()
+    cfg = EfkolosConfig(num_layers=a.layers)
+    dec = BoundedDecoder(DecoderWeights(cfg, max_seq=max(a.prompt, a.budget) + 64), a.sequences, budget=a.budget)
+    g = torch.Generator().manual_seed(0)
+    prompts = torch.randint(0, cfg.vocab_size, (a.sequences, a.prompt), generator=g)
+    dec.generate(prompts, 4, repetition=1.2)  # (first launches)
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    tokens = dec.generate(prompts, a.tokens, repetition=1.2, frequency=0.1)
+    end.record()
+    end.synchronize()
+    ms = start.elapsed_time(end)
+    print(tokens[:, :16].tolist())
+    print(f"{a.sequences} sequences x ({a.prompt} + {a.tokens}) tokens, at most {a.budget + dec.slack} cached: "
+          f"{ms:.1f} ms")
+
+
+if __name__ == "__main__":
+    main()
