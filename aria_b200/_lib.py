@@ -118,6 +118,23 @@ def _lib() -> ctypes.CDLL:
     return _LIB
 
 
+_FAST = None
+
+
+def fastcall():
+    """The C++ binding of the serving operators (aria_b200/_fastcall.so), bound to the
+    library's entry points; like the library it has to have been built."""
+    global _FAST
+    if _FAST is None:
+        import torch  # noqa: F401  (loads what the module links against)
+        from . import _fastcall
+        lib = _lib()
+        _fastcall.bind(*(ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
+            "aria_attention_paged", "aria_prompt_weights", "aria_cache_evict", "aria_logits_adjust")))
+        _FAST = _fastcall
+    return _FAST
+
+
 def lib() -> ctypes.CDLL:
     return _lib()
 

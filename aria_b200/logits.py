@@ -11,8 +11,8 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import BF16, F16, F32, LogitRulesStruct, call
-from .paged import _stream, _want, _workspace
+from ._lib import BF16, F16, F32, LogitRulesStruct, call, fastcall
+from .paged import _NO_WORKSPACE, _WORKSPACES, _stream, _want, _workspace
 
 __all__ = ["adjust", "allowed_mask"]
 
@@ -62,6 +62,14 @@ def adjust(logits: torch.Tensor, *, out: torch.Tensor | None = None, history: to
     Returns (out, token): out of the logits' type (logits itself for in place) or f32;
     token int32 [M] with want_token, else None: the lowest index of the largest f32
     result, -1 where nothing is left above -inf."""
+    if logits.is_cuda:
+        stream = _stream(logits.get_device())
+        ws = _WORKSPACES.get(("logits", logits.get_device(), stream), _NO_WORKSPACE)
+        r = fastcall().logits(ws[0], ws[1], stream, want_token, logits, out, history, history_lens, prompt_lens,
+                              repetition, frequency, presence, bias_tokens, bias_values, allowed, token)
+        if r is not None:
+            return r
+    # the first call on a stream, one that needs more scratch, or something to say
     if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in _DTYPES:
         raise TypeError("logits must be an f32, f16 or bf16 [M][V] CUDA tensor")
     M, V = logits.shape

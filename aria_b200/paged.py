@@ -20,12 +20,13 @@ import math
 import torch
 
 from . import _lib
-from ._lib import BF16, F16, PagedKVStruct, call
+from ._lib import BF16, F16, PagedKVStruct, call, fastcall
 
 __all__ = ["PagedKV", "attention_paged", "prompt_weights", "evict"]
 
 _DTYPES = {torch.float16: F16, torch.bfloat16: BF16}
 _WORKSPACES: dict = {}
+_NO_WORKSPACE = (0, 0, None)
 
 
 # The device's current stream as an integer, without building a Stream object: the
@@ -88,7 +89,7 @@ class PagedKV:
                                 _DTYPES[k_pages.dtype], block_table.data_ptr(),
                                 block_table.stride(0) if M > 1 else block_table.shape[1], block_table.shape[1],
                                 lens.data_ptr())
-        self._ref = ctypes.addressof(self._c)
+        self._ref, self._lens_ptr = ctypes.addressof(self._c), lens.data_ptr()
         self._ws_bytes: dict = {}
 
     def _workspace_bytes(self, heads: int, weights: bool) -> int:
@@ -147,6 +148,14 @@ def attention_paged(q: torch.Tensor, kv: PagedKV, *, k_new: torch.Tensor | None 
     weights f32 [M][kv_heads][cap >= kv.slots]: the running sums of the attention
     weight, updated in place or into weights_out; the new token's slot starts from 0,
     and its entry of slot_pos (int32, the same shape) becomes positions[m]."""
+    stream = _stream(kv.index)
+    ws = _WORKSPACES.get(("attn", kv.index, stream), _NO_WORKSPACE)
+    r = fastcall().attention(kv._ref, kv.M, kv.kv_heads, kv.head_dim, kv.index, kv._scale if scale is None else scale,
+                             ws[0], ws[1], stream, want_lse, q, k_new, v_new, out, weights, weights_out, slot_pos,
+                             positions)
+    if r is not None:
+        return r
+    # the first call on a stream, one that needs more scratch, or something to say
     shape = q.shape
     if len(shape) != 3 or shape[0] != kv.M or shape[2] != kv.head_dim or shape[1] == 0 or shape[1] % kv.kv_heads:
         raise ValueError(f"q must be [{kv.M}][heads][{kv.head_dim}] with heads a multiple of {kv.kv_heads}")
@@ -181,7 +190,6 @@ def attention_paged(q: torch.Tensor, kv: PagedKV, *, k_new: torch.Tensor | None 
             pp = _want(positions, "positions", torch.int32, (kv.M,), dev)
     elif weights_out is not None or slot_pos is not None:
         raise ValueError("weights_out and slot_pos need weights")
-    stream = _stream(dev)
     ws = _workspace("attn", kv._workspace_bytes(heads, wi is not None), dev, stream)
     call("aria_attention_paged", kv._ref, kv.M, heads, q.data_ptr(), qs[0], qs[1], kp, vp, ns[0], ns[1],
          scale if scale is not None else kv._scale, out.data_ptr(), os_[0], os_[1],
@@ -197,6 +205,10 @@ def prompt_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, out: 
     prompt's causal attention returned it.  Writes out[:, :, :T] of an f32
     [B][kv_heads][>= T] tensor with contiguous rows (a new [B][kv_heads][T] one by
     default) and returns it.  head_dim 64 or 128."""
+    if out is not None and q.is_cuda:
+        if fastcall().prompt(q, k, lse, out, scale if scale is not None else 1.0 / math.sqrt(q.shape[-1]), first_query,
+                             _stream(q.get_device())):
+            return out
     if q.dim() != 4 or k.dim() != 4 or q.dtype not in _DTYPES or k.dtype is not q.dtype or not q.is_cuda:
         raise TypeError("q and k must be 4-D f16 or bf16 CUDA tensors of one type")
     B, T, heads, dh = q.shape
@@ -231,21 +243,25 @@ def evict(kv: PagedKV, weights: torch.Tensor, slot_pos: torch.Tensor, next_pos: 
     slots end with weight 0 and position -1.  Returns lens_out (int32 [M], another tensor
     than kv.lens) = min(lens, keep); copy it to kv.lens once every layer that shares kv.lens
     has been evicted from."""
+    if lens_out is None:
+        lens_out = torch.empty_like(kv.lens)
+    dev = kv.index
+    stream = _stream(dev)
+    ws = _WORKSPACES.get(("evict", dev, stream), _NO_WORKSPACE)
+    if fastcall().evict(kv._ref, kv.M, kv.kv_heads, dev, kv._lens_ptr, keep, recent, sinks, ws[0], ws[1], stream, weights,
+                        slot_pos, next_pos, weights_out, slot_pos_out, lens_out):
+        return lens_out
     shape = weights.shape
     if weights.dim() != 3 or shape[:2] != (kv.M, kv.kv_heads):
         raise ValueError("weights must be [M][kv_heads][cap]")
-    dev = kv.index
     wi = _want(weights, "weights", torch.float32, shape, dev)
     pi = _want(slot_pos, "slot_pos", torch.int32, shape, dev)
     wo = wi if weights_out is None else _want(weights_out, "weights_out", torch.float32, shape, dev)
     po = pi if slot_pos_out is None else _want(slot_pos_out, "slot_pos_out", torch.int32, shape, dev)
     npp = _want(next_pos, "next_pos", torch.int32, (kv.M,), dev)
-    if lens_out is None:
-        lens_out = torch.empty_like(kv.lens)
     lp = _want(lens_out, "lens_out", torch.int32, (kv.M,), dev)
     if lp == kv.lens.data_ptr() and kv.M > 0:
         raise ValueError("lens_out must not be kv.lens")
-    stream = _stream(dev)
     ws = _workspace("evict", kv._evict_bytes(keep), dev, stream)
     call("aria_cache_evict", kv._ref, kv.M, wi, wo, pi, po, shape[2], npp, keep, recent, sinks, lp, ws[0], ws[1], stream)
     return lens_out

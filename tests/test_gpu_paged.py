@@ -530,3 +530,61 @@ def test_python_refusals():
         prompt_weights(x, x, torch.zeros(1, 1, 8, device="cuda"))  # head size 32
     with pytest.raises(ValueError):
         prompt_weights(x, x, torch.zeros(1, 1, 7, device="cuda"))
+
+
+# ------------------------------------------------------------------ the two ways from Python
+class _NoFast:
+    def __getattr__(self, name):
+        return lambda *a: None
+
+
+def test_short_and_long_way_agree(monkeypatch):
+    """Every operator through the C++ binding (ctypes forbidden once the workspaces exist) and
+    through ctypes alone: the same bits."""
+    from aria_b200 import logits as lg
+    from aria_b200 import paged
+    g = torch.Generator(device="cuda").manual_seed(1)
+    c = Cache([100, 37, 0], 2, 64, 16, 8, seed=50)
+    q, kn, vn = (torch.randn(3, n, 64, generator=g, device="cuda").half() for n in (4, 2, 2))
+    w0 = torch.rand(3, 2, 130, generator=g, device="cuda")
+    p0 = torch.arange(130, dtype=torch.int32, device="cuda").expand(3, 2, 130).contiguous()
+    pos = c.lens + 9
+    x = torch.randn(1, 50, 2, 64, generator=g, device="cuda").half()
+    lse = torch.randn(1, 2, 50, generator=g, device="cuda") + 5
+    lo = torch.randn(3, 1000, generator=g, device="cuda")
+    hist = torch.randint(0, 1000, (3, 20), generator=g, device="cuda", dtype=torch.int32)
+    n = torch.tensor([20, 3, 0], dtype=torch.int32, device="cuda")
+    r = torch.full((3,), 1.3, device="cuda")
+    bt, bv = hist[:, :4].contiguous(), torch.randn(3, 4, generator=g, device="cuda")
+    mask = lg.allowed_mask(torch.rand(1, 1000, generator=g, device="cuda") < 0.5)
+
+    def everything():
+        w, p, out_w = w0.clone(), p0.clone(), torch.zeros(1, 2, 50, device="cuda")
+        k, v = c.k.clone(), c.v.clone()
+        kv = paged.PagedKV(k, v, c.table, c.lens)
+        res = list(paged.attention_paged(q, kv, k_new=kn, v_new=vn, want_lse=True, weights=w, slot_pos=p, positions=pos))
+        res += paged.attention_paged(q, kv, scale=0.3, out=torch.empty_like(q))[:1]
+        res += [paged.prompt_weights(x, x, lse, out=out_w, first_query=3),
+                paged.evict(kv, w, p, pos, 40, recent=5, sinks=2), w, p, k.nan_to_num(), v.nan_to_num()]
+        res += lg.adjust(lo, history=hist, history_lens=n, prompt_lens=n // 2, repetition=r, frequency=r, presence=r,
+                         bias_tokens=bt, bias_values=bv, allowed=mask, want_token=True)
+        res += lg.adjust(lo, out=torch.empty_like(lo))[:1]
+        torch.cuda.synchronize()
+        return res
+
+    everything()  # the workspaces exist from here on
+
+    def forbidden(*a):
+        raise AssertionError("the long way was taken")
+
+    with monkeypatch.context() as m:
+        m.setattr(paged, "call", forbidden)
+        m.setattr(lg, "call", forbidden)
+        short = everything()
+    with monkeypatch.context() as m:
+        m.setattr(paged, "fastcall", lambda: _NoFast())
+        m.setattr(lg, "fastcall", lambda: _NoFast())
+        long = everything()
+    assert len(short) == len(long)
+    for a, b in zip(short, long):
+        assert torch.equal(a, b)
