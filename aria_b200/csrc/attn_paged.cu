@@ -97,6 +97,9 @@ __device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
@@ -344,6 +347,9 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
     // ---- producer side of this warp's ring: pf is the next tile to load
     PagedCursor pf = seg;
     int left = w1 - w0;
+    constexpr uint32_t kAll = TS == 32 ? 0xffffffffu : (1u << (TS & 31)) - 1u;
+    const int r0 = lane / CPR, ch = lane % CPR;  // this lane's row of a warp-wide copy, and its 16 bytes
+    const long long lane_src = r0 * a.slot_stride + ch * 8, copy_step = RPI * a.slot_stride;
     int page = -1;      // of this lane's rows of that tile (PAGE16: lanes 0-15 its first 16 slots, ...)
     auto page_index = [&](int slot) { return (int)(((unsigned long long)(unsigned)slot * a.page_mul) >> a.page_shift); };
     auto lookup = [&]() {
@@ -377,22 +383,37 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
             rows[h] = pg < 0 ? 0 : min(16, max(0, have - 16 * h));
             valid |= ((1u << rows[h]) - 1u) << (16 * h);
           }
-          if (last < TS) valid |= 1u << last;
-          const int r0 = lane / CPR, ch = lane % CPR;
+          if (valid == kAll && last == TS) {
+            // a whole tile of the pages: one address per half, a constant step per copy
 #pragma unroll
-          for (int i = 0; i < TS * CPR / 32; i++) {
-            const int rh = RPI * i;  // first row of this copy; all of one half
-            const int r = rh + r0, rr = r - (rh & ~15);
-            const bool ok = rr < rows[rh / 16];
-            long long o = ok ? off[rh / 16] + (long long)rr * a.slot_stride + ch * 8 : 0;
-            const uint16_t* kp = a.k_pages + o;
-            const uint16_t* vp = a.v_pages + o;
-            if (r == last) {
-              kp = a.k_new + noff + ch * 8;
-              vp = a.v_new + noff + ch * 8;
+            for (int h = 0; h < HALVES; h++) {
+              const uint16_t* kp = a.k_pages + off[h] + lane_src;
+              const uint16_t* vp = a.v_pages + off[h] + lane_src;
+#pragma unroll
+              for (int i = 16 / RPI * h; i < 16 / RPI * (h + 1); i++) {
+                cp_async_16(dst + tile_off<DH>(RPI * i + r0, ch), kp);
+                cp_async_16(dst + C::kKBytes + tile_off<DH>(RPI * i + r0, ch), vp);
+                kp += copy_step;
+                vp += copy_step;
+              }
             }
-            cp_async_16(dst + tile_off<DH>(r, ch), kp, ok || r == last);
-            cp_async_16(dst + C::kKBytes + tile_off<DH>(r, ch), vp, ok || r == last);
+          } else {
+            if (last < TS) valid |= 1u << last;
+#pragma unroll
+            for (int i = 0; i < TS * CPR / 32; i++) {
+              const int rh = RPI * i;  // first row of this copy; all of one half
+              const int r = rh + r0, rr = r - (rh & ~15);
+              const bool ok = rr < rows[rh / 16];
+              long long o = ok ? off[rh / 16] + (long long)rr * a.slot_stride + ch * 8 : 0;
+              const uint16_t* kp = a.k_pages + o;
+              const uint16_t* vp = a.v_pages + o;
+              if (r == last) {
+                kp = a.k_new + noff + ch * 8;
+                vp = a.v_new + noff + ch * 8;
+              }
+              cp_async_16(dst + tile_off<DH>(r, ch), kp, ok || r == last);
+              cp_async_16(dst + C::kKBytes + tile_off<DH>(r, ch), vp, ok || r == last);
+            }
           }
         } else {
           const int slot = slot0 + lane;
@@ -509,7 +530,6 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
           }
 
         // scores to the log2 domain; slots past the end or without a page are -inf
-        constexpr uint32_t kAll = TS == 32 ? 0xffffffffu : (1u << (TS & 31)) - 1u;
         uint32_t ph[RB][TS / 8], pl[RB][TS / 8];
 #pragma unroll
         for (int rb = 0; rb < RB; rb++) {
