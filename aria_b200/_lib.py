@@ -73,7 +73,9 @@ SIGNATURES = {
     "aria_attention_paged_workspace_bytes": (_SZ, [_P, _I, _I, _I]),
     "aria_attention_paged": (_I, [_P, _I, _I, _P, _L, _L, _P, _P, _L, _L, _F, _P, _L, _L, _P, _P, _P, _L, _P, _P, _P,
                                   _SZ, _P]),
-    "aria_prompt_weights": (_I, [_P, _L, _L, _L, _P, _L, _L, _L, _I, _I, _I, _I, _I, _I, _P, _F, _I, _P, _L, _L, _P]),
+    "aria_prompt_weights": (_I, [_P, _L, _L, _L, _P, _L, _L, _L, _I, _I, _I, _I, _I, _I, _P, _F, _I, _P, _L, _L, _P, _SZ,
+                                 _P]),
+    "aria_prompt_weights_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
     "aria_cache_evict_workspace_bytes": (_SZ, [_P, _I, _I]),
     "aria_cache_evict": (_I, [_P, _I, _P, _P, _P, _P, _L, _P, _I, _I, _I, _P, _P, _SZ, _P]),
     "aria_logits_workspace_bytes": (_SZ, [_I]),

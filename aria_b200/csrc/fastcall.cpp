@@ -139,14 +139,16 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return r;
 }
 
-// q, k, lse, out, scale, first_query, stream
+// q, k, lse, out, scale, first_query, workspace, bytes, stream
 PyObject* prompt(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 7) Py_RETURN_NONE;
+  if (n != 9) Py_RETURN_NONE;
   Args a{args};
   bool bad = false;
   const at::Tensor *q = a.tensor(bad), *k = a.tensor(bad), *lse = a.tensor(bad), *out = a.tensor(bad);
   const float scale = (float)a.real();
   const long long first = a.integer();
+  void* ws = a.pointer();
+  const size_t ws_bytes = (size_t)a.integer();
   void* stream = a.pointer();
   if (PyErr_Occurred()) return nullptr;
   if (bad || !q || !k || !lse || !out || !q->is_cuda() || q->dim() != 4 || k->dim() != 4 || out->dim() != 3 ||
@@ -165,7 +167,7 @@ PyObject* prompt(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int status =
       f_prompt(ptr<const uint16_t>(q), st(q, 0), st(q, 1), st(q, 2), ptr<const uint16_t>(k), st(k, 0), st(k, 1), st(k, 2),
                type_code(type), (int)B, (int)T, (int)heads, (int)kvh, (int)dh, ptr<const float>(lse), scale, (int)first,
-               ptr<float>(out), out->stride(0), out->stride(1), stream);
+               ptr<float>(out), out->stride(0), out->stride(1), ws, ws_bytes, stream);
   if (status != ARIA_Q4_OK) Py_RETURN_NONE;
   Py_RETURN_TRUE;
 }

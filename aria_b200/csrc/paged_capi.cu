@@ -14,7 +14,8 @@ cudaError_t launch_attention_paged(PagedArgs a, int DH, bool bf16, void* ws, con
 cudaError_t launch_prompt_weights(const void* q, const void* k, bool bf16, int DH, long long q_seq, long long q_pos,
                                   long long q_head, long long k_seq, long long k_pos, long long k_head, int B, int T,
                                   int Hkv, int G, int first, float scale, const float* lse, float* w, long long w_seq,
-                                  long long w_head, cudaStream_t st);
+                                  long long w_head, void* ws, cudaStream_t st);
+size_t prompt_workspace_bytes(int B, int T, int Hkv, int G, int first);
 size_t evict_workspace_bytes(int M, int Hkv, long long slots, int keep);
 cudaError_t launch_cache_evict(EvictArgs a, void* ws, cudaStream_t st);
 size_t logits_workspace_bytes(int M);
@@ -106,10 +107,15 @@ int aria_attention_paged(const aria_paged_kv* kv, int M, int heads, const uint16
                                             weights_out, weights_cap, slot_pos, positions, (cudaStream_t)stream));
 }
 
+size_t aria_prompt_weights_workspace_bytes(int B, int T, int heads, int kv_heads, int first_query) {
+  if (B <= 0 || T <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || first_query < 0) return 0;
+  return prompt_workspace_bytes(B, T, kv_heads, heads / kv_heads, first_query);
+}
+
 int aria_prompt_weights(const uint16_t* q, long long q_seq, long long q_pos, long long q_head, const uint16_t* k,
                         long long k_seq, long long k_pos, long long k_head, int dtype, int B, int T, int heads,
                         int kv_heads, int head_dim, const float* lse, float scale, int first_query, float* weights,
-                        long long w_seq, long long w_head, void* stream) {
+                        long long w_seq, long long w_head, void* workspace, size_t workspace_bytes, void* stream) {
   if (B < 0 || T < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || first_query < 0 || !(scale == scale))
     return ARIA_Q4_EINVAL;
   if (dtype != ARIA_Q4_F16 && dtype != ARIA_Q4_BF16) return ARIA_Q4_EINVAL;
@@ -123,11 +129,15 @@ int aria_prompt_weights(const uint16_t* q, long long q_seq, long long q_pos, lon
     if (s % 8) return ARIA_Q4_EALIGN;
     if (s >= (1LL << 38)) return ARIA_Q4_ESIZE;  // the tensor maps' strides are 40 bits of bytes
   }
-  if ((long long)B * kv_heads * ((T + 127) / 128) > 0x7fffffffLL) return ARIA_Q4_ESIZE;
+  if ((long long)B * kv_heads * ((T + 127) / 128) > 0x7fffffffLL / 1024) return ARIA_Q4_ESIZE;
+  if (((uintptr_t)workspace & 255u) != 0) return ARIA_Q4_EALIGN;
   if (int s = check_device()) return s;
+  const size_t need = prompt_workspace_bytes(B, T, kv_heads, heads / kv_heads, first_query);
+  if (need > 0 && !workspace) return ARIA_Q4_EINVAL;
+  if (workspace_bytes < need) return ARIA_Q4_ESIZE;
   return cuda_status(launch_prompt_weights(q, k, dtype == ARIA_Q4_BF16, head_dim, q_seq, q_pos, q_head, k_seq, k_pos,
                                            k_head, B, T, kv_heads, heads / kv_heads, first_query, scale, lse, weights,
-                                           w_seq, w_head, (cudaStream_t)stream));
+                                           w_seq, w_head, workspace, (cudaStream_t)stream));
 }
 
 size_t aria_cache_evict_workspace_bytes(const aria_paged_kv* kv, int M, int keep) {

@@ -18,8 +18,9 @@
 // on the multiply-add pipe instead (558 -> 520 us at that size; two pairs: 531); at 128
 // the added instructions lower the clock by more than they save (597 -> 619).
 //
-// Persistent, one CTA per SM; an item is (sequence, key/value head, key block), the
-// first blocks (most queries) first, dealt out in alternating directions.  Twenty warps:
+// Persistent, one CTA per SM; an item is (sequence, key/value head, key block) or, where
+// those are few, a part of its query blocks (the last part to finish adds the parts' sums
+// in order); the first blocks (most queries) first, dealt out in alternating directions.  Twenty warps:
 //   warp 0      TMA producer: K blocks (two buffers), Q blocks into a ring
 //   warp 1      TMEM allocator and single-thread MMA issuer
 //   warps 2-17  sums: a warp per TMEM lane quadrant and S buffer, so that the four
@@ -34,6 +35,8 @@
 // flag; the code in this unit's g_device_error).
 #include <cuda.h>
 #include <cuda_bf16.h>
+
+#include <algorithm>
 
 #include "q4_common.cuh"
 #include "q4_status.cuh"
@@ -53,6 +56,9 @@ struct PromptArgs {
   float* w;                   // element strides w_seq, w_head
   long long w_seq, w_head;
   int n_kt;                   // key blocks of a sequence
+  int splits;                 // items per (sequence, key/value head, key block)
+  float* parts;               // [item][128] sums, and [item / splits] arrivals (zero between
+  unsigned* arrived;          // calls), where an item is a part of a key block's sums
   unsigned long long wait_ns;
 };
 
@@ -69,7 +75,9 @@ struct PromptSmem {
 };
 
 struct PromptItem {
-  int seq, hk, kt, q0, nq;  // query blocks q0 .. q0 + nq - 1 of each head
+  int seq, hk, kt, q0, nq;  // query blocks q0 .. q0 + nq - 1 of each head, head by head:
+  int lo, hi;               // of these G nq blocks, this item's
+  int index;                // of the item
 };
 // Item of CTA blockIdx.x in round t / gridDim.x (t = blockIdx.x + round * gridDim.x):
 // odd rounds run backwards, so that no CTA has the longer item of every round.
@@ -80,12 +88,26 @@ __device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, int t, in
     t = round * g + (size - 1 - t % g);
   }
   const int bh = a.B * a.Hkv;
+  int base = t, split = 0;
+  if (a.splits > 1) {
+    base = t / a.splits;
+    split = t - base * a.splits;
+  }
   PromptItem r;
-  r.kt = t / bh;
-  r.seq = (t % bh) / a.Hkv;
-  r.hk = t % a.Hkv;
+  r.index = t;
+  r.kt = base / bh;
+  base -= r.kt * bh;
+  r.seq = base / a.Hkv;
+  r.hk = base - r.seq * a.Hkv;
   r.q0 = max(r.kt, a.first / kPwB);
-  r.nq = a.n_kt - r.q0;
+  r.nq = max(0, a.n_kt - r.q0);
+  r.lo = 0;
+  r.hi = a.G * r.nq;
+  if (a.splits > 1) {
+    const long long blocks = r.hi;
+    r.lo = (int)(blocks * split / a.splits);
+    r.hi = (int)(blocks * (split + 1) / a.splits);
+  }
   return r;
 }
 
@@ -161,7 +183,7 @@ __global__ void __launch_bounds__(kPwThreads, 1)
     atomicExch(abort_flag, 1);
   };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n_items = a.n_kt * a.B * a.Hkv;
+  const int n_items = a.n_kt * a.B * a.Hkv * a.splits;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; s++) {
@@ -215,7 +237,7 @@ __global__ void __launch_bounds__(kPwThreads, 1)
       };
       for (int t = blockIdx.x; t < n_items && ok; t += gridDim.x) {
         const PromptItem im = prompt_item(a, t, n_items);
-        if (im.nq <= 0) continue;
+        if (im.lo >= im.hi) continue;
         const int kb = it & 1;
         if (it >= 2 && !wait(&k_empty[kb], ((it >> 1) - 1) & 1)) break;
         tc::mbar_arrive_expect_tx(&k_full[kb], L::kTile);
@@ -224,16 +246,20 @@ __global__ void __launch_bounds__(kPwThreads, 1)
           tc::tma_load_4d(smem + L::kKOff + kb * L::kTile + c * (kPwB * 128), &tm_k, 64 * c, im.hk, im.kt * kPwB,
                           im.seq, &k_full[kb]);
         it++;
-        for (int h = 0; h < a.G && ok; h++)
-          for (int j = 0; j < im.nq; j++, g++) {
-            const int s = g % L::kNQ, use = g / L::kNQ;
-            if (use >= 1 && !wait(&q_empty[s], (use - 1) & 1)) break;
-            tc::mbar_arrive_expect_tx(&q_full[s], L::kTile);
+        int h = im.lo / im.nq, qb = im.lo % im.nq;
+        for (int j = im.lo; j < im.hi; j++, g++) {
+          const int s = g % L::kNQ, use = g / L::kNQ;
+          if (use >= 1 && !wait(&q_empty[s], (use - 1) & 1)) break;
+          tc::mbar_arrive_expect_tx(&q_full[s], L::kTile);
 #pragma unroll
-            for (int c = 0; c < DH / 64; c++)
-              tc::tma_load_4d(smem + L::kQOff + s * L::kTile + c * (kPwB * 128), &tm_q, 64 * c, im.hk * a.G + h,
-                              (im.q0 + j) * kPwB, im.seq, &q_full[s]);
+          for (int c = 0; c < DH / 64; c++)
+            tc::tma_load_4d(smem + L::kQOff + s * L::kTile + c * (kPwB * 128), &tm_q, 64 * c, im.hk * a.G + h,
+                            (im.q0 + qb) * kPwB, im.seq, &q_full[s]);
+          if (++qb == im.nq) {
+            qb = 0;
+            h++;
           }
+        }
       }
       // no copy into shared memory may be in flight when the CTA exits
       for (int i = it > 2 ? it - 2 : 0; i < it; i++) tc::mbar_wait(&k_full[i & 1], (i >> 1) & 1);
@@ -255,11 +281,11 @@ __global__ void __launch_bounds__(kPwThreads, 1)
       int g = 0, it = 0;
       for (int t = blockIdx.x; t < n_items && ok; t += gridDim.x) {
         const PromptItem im = prompt_item(a, t, n_items);
-        if (im.nq <= 0) continue;
+        if (im.lo >= im.hi) continue;
         const int kb = it & 1;
         if (!wait(&k_full[kb], (it >> 1) & 1, tc::kErrTimeoutFull)) break;
         const uint32_t ks = tc::smem_u32(smem + L::kKOff + kb * L::kTile);
-        const int blocks = a.G * im.nq;
+        const int blocks = im.hi - im.lo;
         for (int j = 0; j < blocks; j++, g++) {
           const int s = g % L::kNQ, b = g % kPwS;
           if (!wait(&q_full[s], (g / L::kNQ) & 1, tc::kErrTimeoutFull)) break;
@@ -303,13 +329,16 @@ __global__ void __launch_bounds__(kPwThreads, 1)
     const uint64_t scale2 = pack2(__float_as_uint(a.scale_log2), __float_as_uint(a.scale_log2));
     for (int t = blockIdx.x; t < n_items && ok; t += gridDim.x, it++) {
       const PromptItem im = prompt_item(a, t, n_items);
-      const int key = im.kt * kPwB + r, blocks = im.nq > 0 ? a.G * im.nq : 0;
+      const int key = im.kt * kPwB + r, blocks = im.hi - im.lo;
       const int masked = max(im.kt * kPwB + kPwB - 1, a.first);  // from this query on nothing is left out
       uint64_t sum[2] = {0, 0};  // four running sums
-      for (int j = (b - g0) & (kPwS - 1); j < blocks; j += kPwS, uses++) {
+      int j = (b - g0) & (kPwS - 1);
+      int qb = im.nq > 0 ? (im.lo + j) % im.nq : 0;  // query block of the head
+      for (; j < blocks; j += kPwS, uses++) {
         if (!wait(&s_full[b], uses & 1, tc::kErrTimeoutFull)) break;
         tc::tc_fence_after();
-        const int q0 = (im.q0 + j % im.nq) * kPwB;
+        const int q0 = (im.q0 + qb) * kPwB;
+        for (qb += kPwS; qb >= im.nq;) qb -= im.nq;
         uint32_t sv[2][16];
         tc::tmem_ld_32x32b_x16(s_col, sv[0]);
 #pragma unroll
@@ -396,10 +425,33 @@ __global__ void __launch_bounds__(kPwThreads, 1)
       for (int u = 0; u < kPwB / 32; u++) {
         const int r = 32 * u + lane, key = im.kt * kPwB + r;
         const float sum = (ps[r] + ps[kPwB + r]) + (ps[2 * kPwB + r] + ps[3 * kPwB + r]);
-        if (key < a.T) a.w[(long long)im.seq * a.w_seq + (long long)im.hk * a.w_head + key] = sum;
+        if (a.splits > 1)
+          a.parts[(size_t)im.index * kPwB + r] = sum;
+        else if (key < a.T)
+          a.w[(long long)im.seq * a.w_seq + (long long)im.hk * a.w_head + key] = sum;
       }
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&p_empty[it & 1]);
+      if (a.splits > 1) {  // the key block's last item adds all of them, in order
+        int last = 0;
+        if (lane == 0) {
+          __threadfence();
+          unsigned* arrived = a.arrived + im.index / a.splits;
+          last = atomicAdd(arrived, 1u) == (unsigned)(a.splits - 1);
+          if (last) *arrived = 0;  // ready for the next call
+          __threadfence();
+        }
+        if (__shfl_sync(0xffffffffu, last, 0)) {
+          const float* first = a.parts + (size_t)(im.index - im.index % a.splits) * kPwB;
+#pragma unroll
+          for (int u = 0; u < kPwB / 32; u++) {
+            const int r = 32 * u + lane, key = im.kt * kPwB + r;
+            float sum = 0.0f;
+            for (int k = 0; k < a.splits; k++) sum += __ldcg(first + (size_t)k * kPwB + r);
+            if (key < a.T) a.w[(long long)im.seq * a.w_seq + (long long)im.hk * a.w_head + key] = sum;
+          }
+        }
+      }
     }
   } else if (warp == 2 + kPwSumWarps) {
     // ------------------------------------------------------------ lse rows
@@ -407,29 +459,32 @@ __global__ void __launch_bounds__(kPwThreads, 1)
     bool ok = true;
     for (int t = blockIdx.x; t < n_items && ok; t += gridDim.x) {
       const PromptItem im = prompt_item(a, t, n_items);
-      for (int h = 0; h < a.G && ok; h++) {
+      int h = im.nq > 0 ? im.lo / im.nq : 0, qb = im.lo - h * im.nq;
+      for (int j = im.lo; j < im.hi; j++, g++) {
         const float* row = a.lse + ((size_t)im.seq * a.Hkv * a.G + im.hk * a.G + h) * a.T;
-        for (int j = 0; j < im.nq; j++, g++) {
-          const int b = g % kPwS;
-          float v[4];
+        const int b = g % kPwS;
+        float v[4];
 #pragma unroll
-          for (int u = 0; u < 4; u++) {
-            const int q = (im.q0 + j) * kPwB + 32 * u + lane;
-            v[u] = q < a.T && q >= a.first ? row[q] * -1.4426950408889634f : -INFINITY;
-            if (v[u] == INFINITY) v[u] = -INFINITY;  // a row that saw nothing gives nothing
+        for (int u = 0; u < 4; u++) {
+          const int q = (im.q0 + qb) * kPwB + 32 * u + lane;
+          v[u] = q < a.T && q >= a.first ? row[q] * -1.4426950408889634f : -INFINITY;
+          if (v[u] == INFINITY) v[u] = -INFINITY;  // a row that saw nothing gives nothing
+        }
+        if (g >= kPwS) {
+          const int w = tc::mbar_wait_or_abort(&l_empty[b], ((g / kPwS) - 1) & 1, 2 * a.wait_ns, abort_flag);
+          if (!__all_sync(0xffffffffu, w == tc::kWaitOk)) {
+            if (lane == 0) give_up(w, tc::kErrTimeoutEmpty);
+            ok = false;
+            break;
           }
-          if (g >= kPwS) {
-            const int w = tc::mbar_wait_or_abort(&l_empty[b], ((g / kPwS) - 1) & 1, 2 * a.wait_ns, abort_flag);
-            if (!__all_sync(0xffffffffu, w == tc::kWaitOk)) {
-              if (lane == 0) give_up(w, tc::kErrTimeoutEmpty);
-              ok = false;
-              break;
-            }
-          }
+        }
 #pragma unroll
-          for (int u = 0; u < 4; u++) lse_s[b * kPwB + 32 * u + lane] = v[u];
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(&s_full[b]);
+        for (int u = 0; u < 4; u++) lse_s[b * kPwB + 32 * u + lane] = v[u];
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&s_full[b]);
+        if (++qb == im.nq) {
+          qb = 0;
+          h++;
         }
       }
     }
@@ -481,15 +536,38 @@ static cudaError_t launch_prompt_t(const PromptArgs& a, const CUtensorMap& tq, c
   constexpr auto kern = prompt_weights_kernel<DH, BF16>;
   if (cudaError_t e = allow_smem<kern>(L::kBytes)) return e;
   const int sms = sm_count();
-  const int items = a.n_kt * a.B * a.Hkv;
+  const int items = a.n_kt * a.B * a.Hkv * a.splits;
   kern<<<items < sms ? items : sms, kPwThreads, L::kBytes, st>>>(tq, tk, a);
   return cudaGetLastError();
+}
+
+// Parts that a key block's sums are cut into.  A part costs about as much as 4 blocks
+// (its K block, an empty pipeline, the join), so sums stay whole unless the longest is
+// more than twice an SM's share of all blocks, or 16: then the parts are one and a half
+// such shares.  (One head of 8192 positions, 64 key blocks of 64 to 1: 43 us uncut, 22
+// us cut; 14 heads of 2048, 16 blocks at most: 17 us uncut, 26 cut in two.)
+constexpr int kPwMaxCut = 1024;  // key blocks that may be cut: a fixed number of counters
+static int prompt_splits(int B, int T, int Hkv, int G, int first) {
+  const long long n_kt = (T + kPwB - 1) / kPwB, base = n_kt * B * Hkv;
+  const long long f0 = std::min<long long>(first / kPwB, n_kt), n = n_kt - f0, longest = G * n;
+  if (base > kPwMaxCut) return 1;
+  const long long all = (long long)B * Hkv * G * (f0 * n + n * (n + 1) / 2);
+  const long long share = std::max(8LL, all / sm_count());
+  if (longest <= 2 * share) return 1;
+  return (int)((2 * longest + 3 * share - 1) / (3 * share));
+}
+
+size_t prompt_workspace_bytes(int B, int T, int Hkv, int G, int first) {
+  const int splits = prompt_splits(B, T, Hkv, G, first);
+  if (splits == 1) return 0;
+  const size_t base = (size_t)((T + kPwB - 1) / kPwB) * B * Hkv;
+  return kPwMaxCut * sizeof(unsigned) + base * splits * kPwB * sizeof(float);
 }
 
 cudaError_t launch_prompt_weights(const void* q, const void* k, bool bf16, int DH, long long q_seq, long long q_pos,
                                   long long q_head, long long k_seq, long long k_pos, long long k_head, int B, int T,
                                   int Hkv, int G, int first, float scale, const float* lse, float* w, long long w_seq,
-                                  long long w_head, cudaStream_t st) {
+                                  long long w_head, void* ws, cudaStream_t st) {
   CUtensorMap tq, tk;
   if (!prompt_tmap(&tq, q, bf16, DH, Hkv * G, T, B, q_head, q_pos, q_seq) ||
       !prompt_tmap(&tk, k, bf16, DH, Hkv, T, B, k_head, k_pos, k_seq))
@@ -500,6 +578,9 @@ cudaError_t launch_prompt_weights(const void* q, const void* k, bool bf16, int D
   a.lse = lse;
   a.w = w; a.w_seq = w_seq; a.w_head = w_head;
   a.n_kt = (T + kPwB - 1) / kPwB;
+  a.splits = prompt_splits(B, T, Hkv, G, first);
+  a.arrived = (unsigned*)ws;
+  a.parts = (float*)((uint8_t*)ws + kPwMaxCut * sizeof(unsigned));
   a.wait_ns = tc::kWaitLimitNs;
   if (DH == 64) return bf16 ? launch_prompt_t<64, true>(a, tq, tk, st) : launch_prompt_t<64, false>(a, tq, tk, st);
   if (DH == 128) return bf16 ? launch_prompt_t<128, true>(a, tq, tk, st) : launch_prompt_t<128, false>(a, tq, tk, st);

@@ -206,8 +206,10 @@ def prompt_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, out: 
     [B][kv_heads][>= T] tensor with contiguous rows (a new [B][kv_heads][T] one by
     default) and returns it.  head_dim 64 or 128."""
     if out is not None and q.is_cuda:
+        stream = _stream(q.get_device())
+        ws = _WORKSPACES.get(("prompt", q.get_device(), stream), _NO_WORKSPACE)
         if fastcall().prompt(q, k, lse, out, scale if scale is not None else 1.0 / math.sqrt(q.shape[-1]), first_query,
-                             _stream(q.get_device())):
+                             ws[0], ws[1], stream):
             return out
     if q.dim() != 4 or k.dim() != 4 or q.dtype not in _DTYPES or k.dtype is not q.dtype or not q.is_cuda:
         raise TypeError("q and k must be 4-D f16 or bf16 CUDA tensors of one type")
@@ -227,9 +229,11 @@ def prompt_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, out: 
     if out.dtype is not torch.float32 or out.get_device() != dev or out.dim() != 3 or out.shape[:2] != (B, kvh) or \
             out.shape[2] < T or (out.stride(2) != 1 and out.shape[2] > 1):
         raise ValueError("out must be f32 [B][kv_heads][>= T] with contiguous rows")
+    stream = _stream(dev)
+    ws = _workspace("prompt", _lib.lib().aria_prompt_weights_workspace_bytes(B, T, heads, kvh, first_query), dev, stream)
     call("aria_prompt_weights", q.data_ptr(), qs[0], qs[1], qs[2], k.data_ptr(), ks[0], ks[1], ks[2],
          _DTYPES[q.dtype], B, T, heads, kvh, dh, lp, scale if scale is not None else 1.0 / math.sqrt(dh),
-         first_query, out.data_ptr(), out.stride(0), out.stride(1), _stream(dev))
+         first_query, out.data_ptr(), out.stride(0), out.stride(1), ws[0], ws[1], stream)
     return out
 
 

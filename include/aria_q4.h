@@ -332,11 +332,14 @@ ARIA_Q4_API int aria_attention_paged(const aria_paged_kv* kv, int M, int heads, 
  *                         of exp(scale q[b][t][h].k[b][s][hk] - lse[b][h][t])
  * q, k of dtype with element strides (multiples of 8); lse f32 [B][heads][T]; weights
  * f32 with strides w_seq, w_head; s = 0 .. T - 1 are written.  A row whose lse is
- * -inf gives nothing.  head_dim 64 or 128. */
+ * -inf gives nothing.  head_dim 64 or 128.  workspace as above (0 bytes, NULL, where
+ * no sum is cut; zero-filled before its first use, left ready for calls of any shape). */
+ARIA_Q4_API size_t aria_prompt_weights_workspace_bytes(int B, int T, int heads, int kv_heads, int first_query);
 ARIA_Q4_API int aria_prompt_weights(const uint16_t* q, long long q_seq, long long q_pos, long long q_head,
                                     const uint16_t* k, long long k_seq, long long k_pos, long long k_head, int dtype,
                                     int B, int T, int heads, int kv_heads, int head_dim, const float* lse, float scale,
-                                    int first_query, float* weights, long long w_seq, long long w_head, void* stream);
+                                    int first_query, float* weights, long long w_seq, long long w_head, void* workspace,
+                                    size_t workspace_bytes, void* stream);
 
 /* Eviction.  Every (sequence, key/value head) row with n = lens[m] > keep slots keeps
  * those whose position is >= next_pos[m] - recent or < sinks, then those of the

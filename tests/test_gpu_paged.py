@@ -309,7 +309,7 @@ def test_contiguous_cache_equals_the_decode_attention():
     (1, 1, 1, 1, 64, "f16", 0), (2, 7, 2, 1, 64, "bf16", 3), (1, 127, 1, 2, 128, "f16", 0),
     (1, 128, 2, 1, 64, "f16", 127), (2, 129, 1, 3, 128, "bf16", 128), (1, 300, 3, 1, 64, "f16", 0),
     (3, 260, 2, 2, 64, "f16", 131), (1, 700, 1, 1, 128, "f16", 0), (1, 50, 1, 1, 64, "f16", 50),
-    (1, 40, 1, 1, 64, "f16", 1000)])
+    (1, 40, 1, 1, 64, "f16", 1000), (1, 1000, 1, 4, 64, "f16", 0), (2, 900, 1, 5, 128, "bf16", 200)])
 def test_prompt_weights(B, T, Hkv, G, dh, dtype, first):
     """Lengths around the 128-position block, first queries inside, at and past the end, groups,
     both types, a packed (strided) and a dense layout; slots past T untouched.  Sums of up to

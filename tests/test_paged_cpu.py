@@ -86,12 +86,15 @@ def test_evict_refusals(lib):
 
 
 def test_prompt_refusals(lib):
-    def call(q=256, k=256, s=64, dtype=1, B=1, T=8, heads=2, kvh=1, dh=64, lse=256, scale=0.1, first=0, w=256):
+    def call(q=256, k=256, s=64, dtype=1, B=1, T=8, heads=2, kvh=1, dh=64, lse=256, scale=0.1, first=0, w=256, ws=None):
         return lib.aria_prompt_weights(P(q), s, s, s, P(k), s, s, s, dtype, B, T, heads, kvh, dh, P(lse), scale, first,
-                                       P(w), 8, 8, None)
+                                       P(w), 8, 8, P(ws), 0, None)
     assert call(dh=32) == EUNSUPPORTED and call(dtype=0) == EINVAL and call(kvh=3) == EINVAL
     assert call(first=-1) == EINVAL and call(T=-1) == EINVAL and call(q=None) == EINVAL and call(lse=None) == EINVAL
     assert call(q=264) == EALIGN and call(s=60) == EALIGN and call(s=0) == EINVAL and call(s=1 << 40) == ESIZE
+    assert call(ws=264) == EALIGN
+    size = lib.aria_prompt_weights_workspace_bytes
+    assert size(1, 8, 2, 1, 0) == 0 and size(64, 4096, 14, 14, 0) == 0 and size(1, 8192, 1, 1, 0) > 64 * 512
     assert call(T=0) == OK and call(B=0) == OK and call() in (ECUDA, ENODEVICE)
 
 
