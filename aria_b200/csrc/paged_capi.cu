@@ -34,7 +34,7 @@ static int check_kv(const aria_paged_kv* kv, int M, long long* slots) {
   if (kv->dtype != ARIA_Q4_F16 && kv->dtype != ARIA_Q4_BF16) return ARIA_Q4_EINVAL;
   const int dh = kv->head_dim;
   if (dh != 32 && dh != 64 && dh != 128 && dh != 256) return ARIA_Q4_EUNSUPPORTED;
-  if (M > kPagedMaxSequences) return ARIA_Q4_EUNSUPPORTED;
+  if (M > kPagedMaxSequences || kv->kv_heads > 65535) return ARIA_Q4_EUNSUPPORTED;  // (heads: a grid dimension)
   *slots = (long long)kv->page_size * kv->max_pages;
   if (*slots > kMaxSlots || (long long)M * ((*slots + 15) / 16) > 0x7fffffffLL) return ARIA_Q4_ESIZE;
   if (kv->page_stride % 8 || kv->slot_stride % 8 || kv->head_stride % 8) return ARIA_Q4_EALIGN;
@@ -154,7 +154,7 @@ int aria_cache_evict(const aria_paged_kv* kv, int M, const float* weights_in, fl
   if (keep <= 0 || recent < 0 || sinks < 0 || (long long)recent + sinks > keep) return ARIA_Q4_EINVAL;
   if (cap < slots || slots > kEvictMaxSlots) return ARIA_Q4_ESIZE;
   if (M == 0) return ARIA_Q4_OK;
-  if (!weights_in || !weights_out || !pos_in || !pos_out || !next_pos) return ARIA_Q4_EINVAL;
+  if (!weights_in || !weights_out || !pos_in || !pos_out || !next_pos || lens_out == kv->lens) return ARIA_Q4_EINVAL;
   if ((long long)M * kv->kv_heads > 0x7fffffffLL / 8) return ARIA_Q4_ESIZE;
   const size_t need = evict_workspace_bytes(M, kv->kv_heads, slots, keep);
   if (need > 0 && !workspace) return ARIA_Q4_EINVAL;

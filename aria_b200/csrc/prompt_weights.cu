@@ -134,12 +134,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // 2^x of two values on the multiply-add pipe: x = n + f with n an integer and |f| <= 1/2
 // (n from the low bits of x + 1.5 2^23), a polynomial in f of degree 5 whose coefficients
 // minimise the largest relative error on that interval (Lawson's iteration; 2.3e-7
-// evaluated in f32), and n added to the exponent.  x below -126 gives 2^-126, x above 127
-// gives 2^127, NaN stays NaN.
+// evaluated in f32), and n added to the exponent.  x below -126 gives 0 (-inf does, for
+// masked queries), x above 127 gives 2^127, NaN stays NaN.
 __device__ __forceinline__ uint64_t both(float x) { return pack2(__float_as_uint(x), __float_as_uint(x)); }
 __device__ __forceinline__ void exp2_poly2(float& x, float& y) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-126.0f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(-126.0f));
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(127.0f));
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(127.0f));
   const uint64_t v = pack2(__float_as_uint(x), __float_as_uint(y));
@@ -153,8 +151,8 @@ __device__ __forceinline__ void exp2_poly2(float& x, float& y) {
   float p0, p1, t0, t1;
   unpack2(p, p0, p1);
   unpack2(t, t0, t1);
-  x = __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
-  y = __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
+  x = x < -126.0f ? 0.0f : __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
+  y = y < -126.0f ? 0.0f : __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
 }
 
 template <int DH, bool BF16>

@@ -355,6 +355,19 @@ def test_prompt_weights_rows_that_must_not_count():
     assert np.all(np.abs(got - ref) <= 5e-5 * ref + 1e-6)
 
 
+def test_prompt_weights_of_rows_that_saw_nothing():
+    """Every lse -inf: exactly zero, at both head sizes (their exponentials differ)."""
+    from aria_b200.paged import prompt_weights
+    for dh in (64, 128):
+        q, k = (torch.randn(1, 300, 2, dh, device="cuda").half() for _ in range(2))
+        lse = torch.full((1, 2, 300), -math.inf, device="cuda")
+        assert bool((prompt_weights(q, k, lse) == 0).all())
+        lse[0, 1, 299] = 0.0  # one query counts: exp(scale q.k) of it alone
+        w = prompt_weights(q, k, lse)
+        ref = np.exp(_f64(k[0, :, 1]) @ _f64(q[0, 299, 1]) / math.sqrt(dh))
+        assert bool((w[0, 0] == 0).all()) and np.all(np.abs(_f64(w[0, 1]) - ref) <= 5e-5 * ref + 1e-6)
+
+
 def test_prompt_weights_follow_the_prefill_attention():
     """With the lse of the prompt attention itself, every query's weights add up to 1."""
     from aria_b200.attention import attention_prefill

@@ -75,12 +75,13 @@ def test_workspaces(lib):
 
 def test_evict_refusals(lib):
     def call(kv=None, M=1, wi=256, wo=256, pi=256, po=256, cap=64, nxt=256, keep=32, recent=0, sinks=0, ws=256,
-             nb=1 << 20):
+             nb=1 << 20, lens_out=None):
         kv = _kv() if kv is None else kv
         return lib.aria_cache_evict(ctypes.byref(kv), M, P(wi), P(wo), P(pi), P(po), cap, P(nxt), keep, recent,
-                                    sinks, None, P(ws), nb, None)
+                                    sinks, P(lens_out), P(ws), nb, None)
     assert call(keep=0) == EINVAL and call(recent=-1) == EINVAL and call(recent=30, sinks=3) == EINVAL
     assert call(cap=63) == ESIZE and call(nb=8) == ESIZE and call(ws=None) == EINVAL and call(ws=264) == EALIGN
+    assert call(lens_out=256) == EINVAL  # the lengths themselves
     assert call(wi=None) == EINVAL and call(nxt=None) == EINVAL and call(kv=_kv(head_dim=80)) == EUNSUPPORTED
     assert call(M=0) == OK and call() in (ECUDA, ENODEVICE)
 
