@@ -136,12 +136,15 @@ struct PagedCut {
   }
 };
 
-// One warp: the partial states of the pair at tiles [f, f + nt) of the list -> its
-// output.  offs: shared memory for an int per part that the pair touches.
+// One warp: the partial states of the pair at tiles [f, f + nt) of the list -> rows
+// h_first, h_first + h_step, ... of its output.  offs: shared memory for an int per part
+// that the pair touches.  The loads of a row's first 16 states go out together with
+// those of their maxima and sums: one round trip where a pair has no more.
 template <int DH, int ROWS, bool BF16, bool WEIGHTS>
 __device__ __noinline__ void paged_join(const PagedArgs& a, const PagedCut cut, int f, int nt, int m, int h0,
-                                        int rows, int* offs) {
+                                        int rows, int* offs, int h_first, int h_step) {
   constexpr int VEC = DH >= 128 ? 4 : DH / 32;  // floats per lane and load
+  constexpr int UN = 16;                        // states per batch of loads
   const int lane = threadIdx.x & 31, srows = min(a.G, ROWS), sf = paged_state_floats(DH, srows);
   // the parts' states, in order: a CTA inside the pair has one for all four
   const int p0 = cut.part_of(f), p1 = cut.part_of(f + nt - 1);
@@ -156,57 +159,61 @@ __device__ __noinline__ void paged_join(const PagedArgs& a, const PagedCut cut, 
   }
   __syncwarp();
 #pragma unroll 1
-  for (int h = 0; h < rows; h++) {
-    // every lane's states -> one maximum, the sum of their sums against it
-    float mx = -INFINITY, l = 0.0f;
-    for (int k = lane; k < cnt; k += 32) {
-      const float* st = a.parts + offs[k] + srows * DH + h;
-      const float km = __ldcg(st), kl = __ldcg(st + srows), m2 = fmaxf(mx, km), ms = m2 == -INFINITY ? 0.0f : m2;
-      l = l * paged_ex2(mx - ms) + kl * paged_ex2(km - ms);
-      mx = m2;
-    }
-    float top = mx;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    const float ms = top == -INFINITY ? 0.0f : top;
-    l *= paged_ex2(mx - ms);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  for (int h = h_first; h < rows; h += h_step) {
 #pragma unroll 1
     for (int d0 = lane * VEC; d0 < DH; d0 += 32 * VEC) {
       const float* col = a.parts + h * DH + d0;
+      const float* stat = a.parts + srows * DH + h;
+      float x[UN][VEC];
+      auto load = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < UN; u++) {
+          const float* p = col + offs[min(base + u, cnt - 1)];
+          if (VEC == 4)
+            *reinterpret_cast<float4*>(x[u]) = __ldcg(reinterpret_cast<const float4*>(p));
+          else if (VEC == 2)
+            *reinterpret_cast<float2*>(x[u]) = __ldcg(reinterpret_cast<const float2*>(p));
+          else
+            x[u][0] = __ldcg(p);
+        }
+      };
+      load(0);
+      // every lane's states -> one maximum, the sum of their sums against it
+      float mx = -INFINITY, l = 0.0f;
+      for (int k = lane; k < cnt; k += 32) {
+        const float km = __ldcg(stat + offs[k]), kl = __ldcg(stat + offs[k] + srows), m2 = fmaxf(mx, km);
+        const float ms = m2 == -INFINITY ? 0.0f : m2;
+        l = l * paged_ex2(mx - ms) + kl * paged_ex2(km - ms);
+        mx = m2;
+      }
+      float top = mx;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const float ms = top == -INFINITY ? 0.0f : top;
+      l *= paged_ex2(mx - ms);
+      float w = cnt <= 32 ? paged_ex2(mx - ms) : 0.0f;  // up to 32 states: lane k's maximum is state k's
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
       float acc[VEC];
 #pragma unroll
       for (int v = 0; v < VEC; v++) acc[v] = 0.0f;
-      for (int kb = 0; kb < cnt; kb += 32) {
-        const int todo = min(32, cnt - kb);
-        const float w = lane < todo ? paged_ex2(__ldcg(a.parts + offs[kb + lane] + srows * DH + h) - ms) : 0.0f;
 #pragma unroll 1
-        for (int j = 0; j < todo; j += 16) {  // 16 loads, then their multiply-adds
-          float x[16][VEC];
+      for (int base = 0; base < cnt; base += UN) {
+        if (base > 0) load(base);
+        if (cnt > 32 && base % 32 == 0)
+          w = base + lane < cnt ? paged_ex2(__ldcg(stat + offs[base + lane]) - ms) : 0.0f;
 #pragma unroll
-          for (int u = 0; u < 16; u++) {
-            const float* p = col + offs[kb + min(j + u, todo - 1)];
-            if (VEC == 4)
-              *reinterpret_cast<float4*>(x[u]) = __ldcg(reinterpret_cast<const float4*>(p));
-            else if (VEC == 2)
-              *reinterpret_cast<float2*>(x[u]) = __ldcg(reinterpret_cast<const float2*>(p));
-            else
-              x[u][0] = __ldcg(p);
-          }
+        for (int u = 0; u < UN; u++) {
+          const float wu = __shfl_sync(0xffffffffu, w, base % 32 + u);  // 0 past the last
 #pragma unroll
-          for (int u = 0; u < 16; u++) {
-            const float wu = __shfl_sync(0xffffffffu, w, j + u);  // 0 past the last
-#pragma unroll
-            for (int v = 0; v < VEC; v++) acc[v] = fmaf(wu, x[u][v], acc[v]);
-          }
+          for (int v = 0; v < VEC; v++) acc[v] = fmaf(wu, x[u][v], acc[v]);
         }
       }
 #pragma unroll
       for (int v = 0; v < VEC; v++) paged_store<BF16>(a, m, h0 + h, d0 + v, acc[v] * inv);
+      if (d0 == 0) paged_store_lse<WEIGHTS>(a, m, h0 + h, top, l);
     }
-    if (lane == 0) paged_store_lse<WEIGHTS>(a, m, h0 + h, top, l);
   }
 }
 
@@ -224,7 +231,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
   int* cum = reinterpret_cast<int*>(paged_smem + kPagedWarps * S * C::kStageBytes);  // [M + 1] tiles before m
   int* slots = cum + a.M + 1;                                                       // [M]
   __shared__ int wsum[kPagedWarps];
-  __shared__ int s_maxnt;
+  __shared__ int s_maxnt, s_last;
   __shared__ uint32_t masks[kPagedWarps][kPagedMaxStages];  // per ring stage: the slots that are there
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t4 = lane & 3, mi = lane >> 3, r8 = lane & 7;
@@ -659,7 +666,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
       const PagedCursor p = open[side];
       const int hk = p.hv / a.chunks, h0 = hk * a.G + (p.hv % a.chunks) * ROWS;
       paged_join<DH, ROWS, BF16, WEIGHTS>(a, cut, open_t[side], p.nt, p.m, h0, min(ROWS, (hk + 1) * a.G - h0),
-                                          reinterpret_cast<int*>(ring));
+                                          reinterpret_cast<int*>(ring), 0, 1);
     }
   }
   if (!inside) return;
@@ -701,19 +708,18 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
   }
   if (alone) return;
   __syncthreads();
-  if (warp != 0) return;
-  int last = 0;
-  if (lane == 0) {
+  if (tid == 0) {
     const int p0 = cut.part_of(pair0_t), p1 = cut.part_of(pair0_t + pair0.nt - 1);
     __threadfence();
     unsigned* arrived = a.counters + p0;
-    last = atomicAdd(arrived, (unsigned)kPagedWarps) + kPagedWarps == (unsigned)(p1 - p0 + 1);
-    if (last) *arrived = 0;
+    s_last = atomicAdd(arrived, (unsigned)kPagedWarps) + kPagedWarps == (unsigned)(p1 - p0 + 1);
+    if (s_last) *arrived = 0;
     __threadfence();
   }
-  if (__shfl_sync(0xffffffffu, last, 0))
-    paged_join<DH, ROWS, BF16, WEIGHTS>(a, cut, pair0_t, pair0.nt, pair0.m, h0, rows,
-                                        reinterpret_cast<int*>(ring));
+  __syncthreads();
+  if (s_last)  // the four warps take the rows in turn
+    paged_join<DH, ROWS, BF16, WEIGHTS>(a, cut, pair0_t, pair0.nt, pair0.m, h0, rows, reinterpret_cast<int*>(ring), warp,
+                                        kPagedWarps);
 }
 
 constexpr int kPagedWPT = 4;  // slots per thread
