@@ -79,6 +79,33 @@ def test_adjust_parts(M, hist, biases, grammar):
     _check(M, 517, hist, biases, grammar, "f32", seed=M + hist, prompt=hist != 17)
 
 
+@pytest.mark.parametrize("dtype,out_dtype", [("f32", None), ("f16", None), ("bf16", torch.float32)])
+@pytest.mark.parametrize("hist,biases", [(256, 0), (600, 5), (5000, 100)])
+def test_adjust_long_histories(hist, biases, dtype, out_dtype):
+    """Vocabularies of several chunks with histories around and beyond a block's first
+    load; odd sizes, out of place and in place."""
+    _check(3, 40001, hist, biases, True, dtype, out_dtype, seed=hist)
+    _check(2, 33000, hist, biases, False, dtype, seed=hist + 1, pad=3, in_place=True, prompt=False)
+
+
+def test_adjust_counts_beyond_15_bits():
+    """Histories longer than a 15-bit count holds: forty tokens a thousand times each."""
+    from aria_b200.logits import adjust
+    M, V, H = 2, 50001, 40000
+    x = torch.randn(M, V, device="cuda") * 3
+    hist = torch.randint(0, 40, (M, H), dtype=torch.int32, device="cuda")
+    hist[0, :33000] = 7  # one of them more than 32767 times
+    n = torch.tensor([H, 300], dtype=torch.int32, device="cuda")
+    f = torch.tensor([0.001, 0.01], device="cuda")
+    a, token = adjust(x, history=hist, history_lens=n, frequency=f, repetition=f + 1, want_token=True)
+    assert torch.equal(token.long(), a.argmax(1))
+    for m in range(M):
+        count = torch.bincount(hist[m, :int(n[m])], minlength=V).double()
+        y, r, w = x[m].double(), 1 + f[m].double(), f[m].double()
+        ref = torch.where(count > 0, torch.where(y > 0, y / r, y * r), y) - w * count
+        assert (a[m].double() - ref).abs().max().item() <= 3e-5  # (f32: 33 + 15 at most)
+
+
 def test_adjust_rows_in_place_and_shared_mask():
     _check(4, 1003, 50, 3, True, "f16", seed=1, pad=5, in_place=True, shared_mask=True)
     _check(4, 5001, 50, 33, True, "f32", seed=2, pad=7)
