@@ -70,6 +70,7 @@ SIGNATURES = {
     "aria_attention_decode": (_I, [_P, _I, _I, _I, _P, _P, _I, _P, _P, _P]),
     "aria_flash_attn_fwd": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _F, _P]),
     "aria_attention_prefill": (_I, [_P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P]),
+    "aria_paged_workspace_counter_bytes": (_SZ, []),
     "aria_attention_paged_workspace_bytes": (_SZ, [_P, _I, _I, _I]),
     "aria_attention_paged": (_I, [_P, _I, _I, _P, _L, _L, _P, _P, _L, _L, _F, _P, _L, _L, _P, _P, _P, _L, _P, _P, _P,
                                   _SZ, _P]),
@@ -89,6 +90,7 @@ SIGNATURES = {
     "aria_q4_strerror": (ctypes.c_char_p, [_I]),
     "aria_q4_last_cuda_error": (_I, []),
     "aria_q4_take_device_error": (_I, []),
+    "aria_stream_capture_id": (_I, [_P, _P]),
     "aria_q4_abi_version": (_I, []),
 }
 

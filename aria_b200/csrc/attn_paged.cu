@@ -779,7 +779,7 @@ static size_t paged_part_bytes(int DH, int G) {
 // Workspace: one counter per warp (zero between calls; a region of fixed size, so
 // that calls of any shape may follow one another), partial states, and for the
 // accumulated weights one log-sum-exp and score_row scores per query head.
-static size_t paged_counter_bytes() { return align_up((size_t)paged_grid() * kPagedWarps * sizeof(unsigned), 256); }
+size_t paged_counter_bytes() { return align_up((size_t)paged_grid() * kPagedWarps * sizeof(unsigned), 256); }
 
 size_t paged_workspace_bytes(int M, int Hq, int Hkv, int DH, long long slots, bool weights) {
   const int G = Hq / Hkv;

@@ -8,6 +8,8 @@
 #include "q4_status.cuh"
 
 namespace aria_q4 {
+size_t paged_counter_bytes();
+size_t prompt_counter_bytes();
 size_t paged_workspace_bytes(int M, int Hq, int Hkv, int DH, long long slots, bool weights);
 cudaError_t launch_attention_paged(PagedArgs a, int DH, bool bf16, void* ws, const float* win, float* wout,
                                    long long cap, int* slot_pos, const int* positions, cudaStream_t st);
@@ -45,6 +47,21 @@ static int check_kv(const aria_paged_kv* kv, int M, long long* slots) {
 }
 
 extern "C" {
+
+size_t aria_paged_workspace_counter_bytes(void) {
+  const size_t a = paged_counter_bytes(), b = prompt_counter_bytes();
+  return a > b ? a : b;
+}
+
+int aria_stream_capture_id(void* stream, unsigned long long* id) {
+  if (!id) return ARIA_Q4_EINVAL;
+  *id = 0;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long of = 0;
+  if (cudaError_t e = cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &of)) return cuda_status(e);
+  if (status == cudaStreamCaptureStatusActive) *id = of;
+  return ARIA_Q4_OK;
+}
 
 size_t aria_attention_paged_workspace_bytes(const aria_paged_kv* kv, int M, int heads, int weights) {
   long long slots = 0;

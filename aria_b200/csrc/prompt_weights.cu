@@ -555,11 +555,13 @@ static int prompt_splits(int B, int T, int Hkv, int G, int first) {
   return (int)((2 * longest + 3 * share - 1) / (3 * share));
 }
 
+size_t prompt_counter_bytes() { return kPwMaxCut * sizeof(unsigned); }
+
 size_t prompt_workspace_bytes(int B, int T, int Hkv, int G, int first) {
   const int splits = prompt_splits(B, T, Hkv, G, first);
   if (splits == 1) return 0;
   const size_t base = (size_t)((T + kPwB - 1) / kPwB) * B * Hkv;
-  return kPwMaxCut * sizeof(unsigned) + base * splits * kPwB * sizeof(float);
+  return prompt_counter_bytes() + base * splits * kPwB * sizeof(float);
 }
 
 cudaError_t launch_prompt_weights(const void* q, const void* k, bool bf16, int DH, long long q_seq, long long q_pos,
@@ -578,7 +580,7 @@ cudaError_t launch_prompt_weights(const void* q, const void* k, bool bf16, int D
   a.n_kt = (T + kPwB - 1) / kPwB;
   a.splits = prompt_splits(B, T, Hkv, G, first);
   a.arrived = (unsigned*)ws;
-  a.parts = (float*)((uint8_t*)ws + kPwMaxCut * sizeof(unsigned));
+  a.parts = (float*)((uint8_t*)ws + prompt_counter_bytes());
   a.wait_ns = tc::kWaitLimitNs;
   if (DH == 64) return bf16 ? launch_prompt_t<64, true>(a, tq, tk, st) : launch_prompt_t<64, false>(a, tq, tk, st);
   if (DH == 128) return bf16 ? launch_prompt_t<128, true>(a, tq, tk, st) : launch_prompt_t<128, false>(a, tq, tk, st);

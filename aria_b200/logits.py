@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from ._lib import BF16, F16, F32, LogitRulesStruct, call, fastcall
-from .paged import _NO_WORKSPACE, _WORKSPACES, _stream, _want, _workspace
+from .paged import _held, _stream, _want, _workspace
 
 __all__ = ["adjust", "allowed_mask"]
 
@@ -64,7 +64,7 @@ def adjust(logits: torch.Tensor, *, out: torch.Tensor | None = None, history: to
     result, -1 where nothing is left above -inf."""
     if logits.is_cuda:
         stream = _stream(logits.get_device())
-        ws = _WORKSPACES.get(("logits", logits.get_device(), stream), _NO_WORKSPACE)
+        ws = _held("logits", logits.get_device(), stream)
         r = fastcall().logits(ws[0], ws[1], stream, want_token, logits, out, history, history_lens, prompt_lens,
                               repetition, frequency, presence, bias_tokens, bias_values, allowed, token)
         if r is not None:
@@ -123,7 +123,7 @@ def adjust(logits: torch.Tensor, *, out: torch.Tensor | None = None, history: to
         if token is None:
             token = torch.empty(rows, dtype=i32, device=logits.device)
         tp = _want(token, "token", i32, rows, dev)
-        ws = _workspace("logits", _ws_bytes(M), dev, stream)
+        ws = _workspace("logits", _ws_bytes(M), dev, stream, "all")
     call("aria_logits_adjust", ctypes.addressof(r), logits.data_ptr(), _DTYPES[logits.dtype], x_row, M, V,
          out.data_ptr(), _DTYPES[out.dtype], y_row, tp, ws[0], ws[1], stream)
     return out, token

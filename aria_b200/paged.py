@@ -25,23 +25,50 @@ from ._lib import BF16, F16, PagedKVStruct, call, fastcall
 __all__ = ["PagedKV", "attention_paged", "prompt_weights", "evict"]
 
 _DTYPES = {torch.float16: F16, torch.bfloat16: BF16}
+# (operator, device, stream) -> (pointer, bytes, tensor): scratch of eager calls, and of the
+# calls of the graph that was captured last on the stream (with the capture's id)
 _WORKSPACES: dict = {}
+_GRAPH_WORKSPACES: dict = {}
 _NO_WORKSPACE = (0, 0, None)
 
 
 # The device's current stream as an integer, without building a Stream object: the
 # host's part of a call is a few microseconds in all.
 _stream = torch._C._cuda_getCurrentRawStream
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
-def _workspace(kind: str, nbytes: int, dev: int, stream: int) -> tuple:
-    """(pointer, bytes, tensor) of zero-filled scratch of one operator on this device
-    and stream, grown on demand; every call leaves it ready for the next."""
-    key = (kind, dev, stream)
-    ws = _WORKSPACES.get(key)
-    if ws is None or ws[1] < nbytes:
-        t = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", dev))
-        ws = _WORKSPACES[key] = (t.data_ptr(), t.numel(), t)
+def _capture_id(stream: int) -> int:
+    n = ctypes.c_ulonglong(0)
+    call("aria_stream_capture_id", stream, ctypes.addressof(n))
+    return n.value
+
+
+def _held(kind: str, dev: int, stream: int) -> tuple:
+    """The scratch of one operator that exists for a call made now, or _NO_WORKSPACE.
+
+    A captured graph keeps the addresses of its calls, so it shares no scratch with eager
+    calls (which replace theirs when they need more) nor with another graph."""
+    if _capturing():
+        ws = _GRAPH_WORKSPACES.get((kind, dev, stream))
+        return ws if ws is not None and ws[3] == _capture_id(stream) else _NO_WORKSPACE
+    return _WORKSPACES.get((kind, dev, stream), _NO_WORKSPACE)
+
+
+def _workspace(kind: str, nbytes: int, dev: int, stream: int, cleared: str = "counters") -> tuple:
+    """(pointer, bytes, tensor) of scratch of one operator on this device and stream; when it
+    is new its counters ("counters": those at the start; "all": every byte may be one) are
+    zero.  Grown on demand, and left by every call as the next one, of any size, needs it.
+    Within a capture it is allocated from the graph's pool, which lives as long as the
+    graph, and cleared by the graph itself."""
+    ws = _held(kind, dev, stream)
+    if ws[2] is None or ws[1] < nbytes:
+        t = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", dev))
+        t[:_lib.lib().aria_paged_workspace_counter_bytes() if cleared == "counters" else None].zero_()
+        if _capturing():
+            ws = _GRAPH_WORKSPACES[kind, dev, stream] = (t.data_ptr(), t.numel(), t, _capture_id(stream))
+        else:
+            ws = _WORKSPACES[kind, dev, stream] = (t.data_ptr(), t.numel(), t)
     return ws
 
 
@@ -149,7 +176,7 @@ def attention_paged(q: torch.Tensor, kv: PagedKV, *, k_new: torch.Tensor | None 
     weight, updated in place or into weights_out; the new token's slot starts from 0,
     and its entry of slot_pos (int32, the same shape) becomes positions[m]."""
     stream = _stream(kv.index)
-    ws = _WORKSPACES.get(("attn", kv.index, stream), _NO_WORKSPACE)
+    ws = _held("attn", kv.index, stream)
     r = fastcall().attention(kv._ref, kv.M, kv.kv_heads, kv.head_dim, kv.index, kv._scale if scale is None else scale,
                              ws[0], ws[1], stream, want_lse, q, k_new, v_new, out, weights, weights_out, slot_pos,
                              positions)
@@ -207,7 +234,7 @@ def prompt_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, out: 
     default) and returns it.  head_dim 64 or 128."""
     if out is not None and q.is_cuda:
         stream = _stream(q.get_device())
-        ws = _WORKSPACES.get(("prompt", q.get_device(), stream), _NO_WORKSPACE)
+        ws = _held("prompt", q.get_device(), stream)
         if fastcall().prompt(q, k, lse, out, scale if scale is not None else 1.0 / math.sqrt(q.shape[-1]), first_query,
                              ws[0], ws[1], stream):
             return out
@@ -251,7 +278,7 @@ def evict(kv: PagedKV, weights: torch.Tensor, slot_pos: torch.Tensor, next_pos: 
         lens_out = torch.empty_like(kv.lens)
     dev = kv.index
     stream = _stream(dev)
-    ws = _WORKSPACES.get(("evict", dev, stream), _NO_WORKSPACE)
+    ws = _held("evict", dev, stream)
     if fastcall().evict(kv._ref, kv.M, kv.kv_heads, dev, kv._lens_ptr, keep, recent, sinks, ws[0], ws[1], stream, weights,
                         slot_pos, next_pos, weights_out, slot_pos_out, lens_out):
         return lens_out

@@ -314,9 +314,12 @@ typedef struct {
  *     weights_out[m][hk][j] = weights_in[m][hk][j] + sum over the group's heads of p_j
  * where the new token's slot counts from 0; with slot_pos (int, same shape) and
  * positions (int [M]) that slot's entry becomes positions[m].
- * workspace: aria_attention_paged_workspace_bytes, 256-byte aligned, zero-filled
- * before its first use; every call of any shape leaves it ready for the next.
- * Calls that share one must be ordered. */
+ * workspace: aria_attention_paged_workspace_bytes, 256-byte aligned, its first
+ * aria_paged_workspace_counter_bytes zero before its first use; every call of any
+ * shape leaves it ready for the next.  Calls that share one must be ordered, and a
+ * captured graph's workspace lives as long as the graph: give each graph its own,
+ * cleared on the captured stream before its first call. */
+ARIA_Q4_API size_t aria_paged_workspace_counter_bytes(void);
 ARIA_Q4_API size_t aria_attention_paged_workspace_bytes(const aria_paged_kv* kv, int M, int heads, int weights);
 ARIA_Q4_API int aria_attention_paged(const aria_paged_kv* kv, int M, int heads, const uint16_t* q, long long q_row,
                                      long long q_head, const uint16_t* k_new, const uint16_t* v_new,
@@ -333,7 +336,8 @@ ARIA_Q4_API int aria_attention_paged(const aria_paged_kv* kv, int M, int heads, 
  * q, k of dtype with element strides (multiples of 8); lse f32 [B][heads][T]; weights
  * f32 with strides w_seq, w_head; s = 0 .. T - 1 are written.  A row whose lse is
  * -inf gives nothing.  head_dim 64 or 128.  workspace as above (0 bytes, NULL, where
- * no sum is cut; zero-filled before its first use, left ready for calls of any shape). */
+ * no sum is cut); after a call during which a bounded wait expired
+ * (aria_q4_take_device_error() != 0) its counters have to be cleared again. */
 ARIA_Q4_API size_t aria_prompt_weights_workspace_bytes(int B, int T, int heads, int kv_heads, int first_query);
 ARIA_Q4_API int aria_prompt_weights(const uint16_t* q, long long q_seq, long long q_pos, long long q_head,
                                     const uint16_t* k, long long k_seq, long long k_pos, long long k_head, int dtype,
@@ -446,6 +450,9 @@ enum {
  * shared by every stream and thread.  Synchronises the device.  No reference
  * counterpart (the reference aborts). */
 ARIA_Q4_API int aria_q4_take_device_error(void);
+/* The id of the graph capture that `stream` is part of (unique in the process), 0 when
+ * it is not being captured: tells one graph's workspaces from another's. */
+ARIA_Q4_API int aria_stream_capture_id(void* stream, unsigned long long* id);
 ARIA_Q4_API int aria_q4_abi_version(void);
 
 /* ---------------------------------------------------------------- test hook */
