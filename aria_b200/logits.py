@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from ._lib import BF16, F16, F32, LogitRulesStruct, call, fastcall
-from .paged import _held, _stream, _want, _workspace
+from .paged import _current_device, _held, _stream, _want, _workspace
 
 __all__ = ["adjust", "allowed_mask"]
 
@@ -63,6 +63,11 @@ def adjust(logits: torch.Tensor, *, out: torch.Tensor | None = None, history: to
     token int32 [M] with want_token, else None: the lowest index of the largest f32
     result, -1 where nothing is left above -inf."""
     if logits.is_cuda:
+        if _current_device() != logits.get_device():  # a launch goes to the current device
+            with torch.cuda.device(logits.get_device()):
+                return adjust(logits, out=out, history=history, history_lens=history_lens, prompt_lens=prompt_lens,
+                              repetition=repetition, frequency=frequency, presence=presence, bias_tokens=bias_tokens,
+                              bias_values=bias_values, allowed=allowed, want_token=want_token, token=token)
         stream = _stream(logits.get_device())
         ws = _held("logits", logits.get_device(), stream)
         r = fastcall().logits(ws[0], ws[1], stream, want_token, logits, out, history, history_lens, prompt_lens,

@@ -9,8 +9,8 @@ weight its slots have received, and eviction by that weight (libaria_q4.so).
 The reference's cache (KVCache, lold3344/ARIA src/transformer_cuda.rs:144-155) is
 contiguous and grows with the sequence; paging and eviction have no counterpart
 there.  No fallback: without the library or a B200 every call raises.  Calls run
-on the current stream of the tensors' device; what they write in place, they write
-in the order of that stream.
+on the current stream of the tensors' device, whichever device is current; what they
+write in place, they write in the order of that stream.
 """
 from __future__ import annotations
 
@@ -36,6 +36,7 @@ _NO_WORKSPACE = (0, 0, None)
 # host's part of a call is a few microseconds in all.
 _stream = torch._C._cuda_getCurrentRawStream
 _capturing = torch._C._cuda_isCurrentStreamCapturing
+_current_device = torch._C._cuda_getDevice
 
 
 def _capture_id(stream: int) -> int:
@@ -175,6 +176,10 @@ def attention_paged(q: torch.Tensor, kv: PagedKV, *, k_new: torch.Tensor | None 
     weights f32 [M][kv_heads][cap >= kv.slots]: the running sums of the attention
     weight, updated in place or into weights_out; the new token's slot starts from 0,
     and its entry of slot_pos (int32, the same shape) becomes positions[m]."""
+    if _current_device() != kv.index:  # a launch goes to the current device
+        with torch.cuda.device(kv.index):
+            return attention_paged(q, kv, k_new=k_new, v_new=v_new, scale=scale, out=out, want_lse=want_lse,
+                                   weights=weights, weights_out=weights_out, slot_pos=slot_pos, positions=positions)
     stream = _stream(kv.index)
     ws = _held("attn", kv.index, stream)
     r = fastcall().attention(kv._ref, kv.M, kv.kv_heads, kv.head_dim, kv.index, kv._scale if scale is None else scale,
@@ -232,6 +237,9 @@ def prompt_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, out: 
     prompt's causal attention returned it.  Writes out[:, :, :T] of an f32
     [B][kv_heads][>= T] tensor with contiguous rows (a new [B][kv_heads][T] one by
     default) and returns it.  head_dim 64 or 128."""
+    if q.is_cuda and _current_device() != q.get_device():
+        with torch.cuda.device(q.get_device()):
+            return prompt_weights(q, k, lse, out=out, scale=scale, first_query=first_query)
     if out is not None and q.is_cuda:
         stream = _stream(q.get_device())
         ws = _held("prompt", q.get_device(), stream)
@@ -274,6 +282,10 @@ def evict(kv: PagedKV, weights: torch.Tensor, slot_pos: torch.Tensor, next_pos: 
     slots end with weight 0 and position -1.  Returns lens_out (int32 [M], another tensor
     than kv.lens) = min(lens, keep); copy it to kv.lens once every layer that shares kv.lens
     has been evicted from."""
+    if _current_device() != kv.index:
+        with torch.cuda.device(kv.index):
+            return evict(kv, weights, slot_pos, next_pos, keep, recent=recent, sinks=sinks, weights_out=weights_out,
+                         slot_pos_out=slot_pos_out, lens_out=lens_out)
     if lens_out is None:
         lens_out = torch.empty_like(kv.lens)
     dev = kv.index

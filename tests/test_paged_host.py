@@ -50,3 +50,62 @@ def test_capture_id_refuses_nothing_to_write():
     from aria_b200 import _lib
     assert _lib.lib().aria_stream_capture_id(None, None) == _lib.EINVAL
     assert _lib.lib().aria_paged_workspace_counter_bytes() >= 4 * 2 * 148 * 4
+
+
+class _OnDevice1:
+    """A tensor of cuda:1, as far as the entry points look before they call the library."""
+    is_cuda, shape = True, (1, 1, 1, 64)
+
+    def get_device(self):
+        return 1
+
+
+def test_calls_are_made_with_the_tensors_device_current(monkeypatch):
+    """cuda:0 is current, the tensors are on cuda:1: every call is made, with every argument it was
+    given, while cuda:1 is current, and cuda:0 is current again afterwards."""
+    import contextlib
+    import types
+
+    from aria_b200 import logits
+    state = {"device": 0, "calls": []}
+
+    @contextlib.contextmanager
+    def device(i):
+        before, state["device"] = state["device"], i
+        yield
+        state["device"] = before
+
+    class Fast:
+        def __getattr__(self, name):
+            def record(*args):
+                state["calls"].append((name, state["device"], args))
+                return "made"
+            return record
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    for module in (paged, logits):
+        monkeypatch.setattr(module, "_current_device", lambda: state["device"])
+        monkeypatch.setattr(module, "_stream", lambda i: 100 + i)
+        monkeypatch.setattr(module, "_held", lambda kind, dev, stream: (0, 0, None))
+        monkeypatch.setattr(module, "fastcall", Fast)
+    kv = types.SimpleNamespace(_ref=1, M=1, kv_heads=1, head_dim=64, index=1, _scale=0.1, _lens_ptr=2)
+    t = _OnDevice1()
+    args = [object() for _ in range(12)]
+    for current in (0, 1):
+        state.update(device=current, calls=[])
+        assert paged.attention_paged(args[0], kv, k_new=args[1], v_new=args[2], scale=0.5, out=args[3], want_lse=True,
+                                     weights=args[4], weights_out=args[5], slot_pos=args[6],
+                                     positions=args[7]) == "made"
+        assert paged.prompt_weights(t, args[0], args[1], out=args[2], scale=0.5, first_query=7) is args[2]
+        assert paged.evict(kv, args[0], args[1], args[2], 9, recent=3, sinks=2, weights_out=args[3], slot_pos_out=args[4],
+                           lens_out=args[5]) is args[5]
+        assert logits.adjust(t, out=args[0], history=args[1], history_lens=args[2], prompt_lens=args[3],
+                             repetition=args[4], frequency=args[5], presence=args[6], bias_tokens=args[7],
+                             bias_values=args[8], allowed=args[9], want_token=True, token=args[10]) == "made"
+        assert [(n, d) for n, d, _ in state["calls"]] == [("attention", 1), ("prompt", 1), ("evict", 1), ("logits", 1)]
+        assert state["device"] == current
+        attention, prompt, evict, adjust = (c[2] for c in state["calls"])
+        assert attention == (1, 1, 1, 64, 1, 0.5, 0, 0, 101, True, *args[:8])
+        assert prompt == (t, args[0], args[1], args[2], 0.5, 7, 0, 0, 101)
+        assert evict == (1, 1, 1, 1, 2, 9, 3, 2, 0, 0, 101, *args[:6])
+        assert adjust == (0, 0, 101, True, t, *args[:11])
