@@ -62,23 +62,24 @@ def adjust(logits: torch.Tensor, *, out: torch.Tensor | None = None, history: to
     Returns (out, token): out of the logits' type (logits itself for in place) or f32;
     token int32 [M] with want_token, else None: the lowest index of the largest f32
     result, -1 where nothing is left above -inf."""
-    if logits.is_cuda:
-        if _current_device() != logits.get_device():  # a launch goes to the current device
-            with torch.cuda.device(logits.get_device()):
+    dev = logits.get_device()  # -1 on the CPU
+    if dev >= 0:
+        if _current_device() != dev:  # a launch goes to the current device
+            with torch.cuda.device(dev):
                 return adjust(logits, out=out, history=history, history_lens=history_lens, prompt_lens=prompt_lens,
                               repetition=repetition, frequency=frequency, presence=presence, bias_tokens=bias_tokens,
                               bias_values=bias_values, allowed=allowed, want_token=want_token, token=token)
-        stream = _stream(logits.get_device())
-        ws = _held("logits", logits.get_device(), stream)
+        stream = _stream(dev)
+        ws = _held("logits", dev, stream)
         r = fastcall().logits(ws[0], ws[1], stream, want_token, logits, out, history, history_lens, prompt_lens,
                               repetition, frequency, presence, bias_tokens, bias_values, allowed, token)
         if r is not None:
             return r
     # the first call on a stream, one that needs more scratch, or something to say
-    if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in _DTYPES:
+    if dev < 0 or logits.dim() != 2 or logits.dtype not in _DTYPES:
         raise TypeError("logits must be an f32, f16 or bf16 [M][V] CUDA tensor")
     M, V = logits.shape
-    dev, i32, f32, rows = logits.get_device(), torch.int32, torch.float32, (M,)
+    i32, f32, rows = torch.int32, torch.float32, (M,)
     x_row = _matrix(logits, "logits", logits.dtype, M, dev)
     if out is None:
         out = torch.empty((M, V), dtype=logits.dtype, device=logits.device)

@@ -50,7 +50,7 @@ def _held(kind: str, dev: int, stream: int) -> tuple:
 
     A captured graph keeps the addresses of its calls, so it shares no scratch with eager
     calls (which replace theirs when they need more) nor with another graph."""
-    if _capturing():
+    if stream != 0 and _capturing():  # (the default stream cannot be captured)
         ws = _GRAPH_WORKSPACES.get((kind, dev, stream))
         return ws if ws is not None and ws[3] == _capture_id(stream) else _NO_WORKSPACE
     return _WORKSPACES.get((kind, dev, stream), _NO_WORKSPACE)
@@ -237,19 +237,20 @@ def prompt_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, out: 
     prompt's causal attention returned it.  Writes out[:, :, :T] of an f32
     [B][kv_heads][>= T] tensor with contiguous rows (a new [B][kv_heads][T] one by
     default) and returns it.  head_dim 64 or 128."""
-    if q.is_cuda and _current_device() != q.get_device():
-        with torch.cuda.device(q.get_device()):
+    dev = q.get_device()  # -1 on the CPU
+    if dev >= 0 and _current_device() != dev:
+        with torch.cuda.device(dev):
             return prompt_weights(q, k, lse, out=out, scale=scale, first_query=first_query)
-    if out is not None and q.is_cuda:
-        stream = _stream(q.get_device())
-        ws = _held("prompt", q.get_device(), stream)
+    if out is not None and dev >= 0:
+        stream = _stream(dev)
+        ws = _held("prompt", dev, stream)
         if fastcall().prompt(q, k, lse, out, scale if scale is not None else 1.0 / math.sqrt(q.shape[-1]), first_query,
                              ws[0], ws[1], stream):
             return out
     if q.dim() != 4 or k.dim() != 4 or q.dtype not in _DTYPES or k.dtype is not q.dtype or not q.is_cuda:
         raise TypeError("q and k must be 4-D f16 or bf16 CUDA tensors of one type")
     B, T, heads, dh = q.shape
-    kvh, dev = k.shape[2], q.get_device()
+    kvh = k.shape[2]
     if k.shape != (B, T, kvh, dh) or k.get_device() != dev or kvh == 0 or heads % kvh:
         raise ValueError("k must be [B][T][kv_heads][dh] with heads a multiple of kv_heads")
     qs, ks = q.stride(), k.stride()
