@@ -242,10 +242,12 @@ int aria_logits_adjust(const aria_logit_rules* r, const void* logits, int dtype,
   a.repetition = r->repetition;
   a.frequency = r->frequency;
   a.presence = r->presence;
-  a.bias_tokens = r->biases > 0 ? r->bias_tokens : nullptr;
-  a.bias_values = r->bias_values;
-  a.bias_row = r->bias_row;
-  a.biases = r->biases;
+  if (r->bias_tokens && r->biases > 0) {  // without the list its length says nothing
+    a.bias_tokens = r->bias_tokens;
+    a.bias_values = r->bias_values;
+    a.bias_row = r->bias_row;
+    a.biases = r->biases;
+  }
   a.allowed = r->allowed;
   a.allowed_row = r->allowed_row;
   a.token = token;
