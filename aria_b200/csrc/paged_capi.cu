@@ -1,6 +1,8 @@
 // paged_capi.cu -- extern "C" entry points of the paged KV cache and of the logits
 // (declared in include/aria_q4.h): argument checks and status codes; the kernels
 // live in attn_paged.cu, prompt_weights.cu, cache_evict.cu and logits.cu.
+#include <initializer_list>
+
 #include "../../include/aria_q4.h"
 #include "q4_common.cuh"
 #include "q4_logits.cuh"
@@ -28,6 +30,13 @@ using namespace aria_q4;
 
 static const long long kMaxSlots = 0x7fffff00;   // of one sequence
 
+// whether every pointer is a multiple of n bytes (its element's size; NULL is)
+static bool elements_aligned(size_t n, std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if ((uintptr_t)p % n) return false;
+  return true;
+}
+
 static int check_kv(const aria_paged_kv* kv, int M, long long* slots) {
   if (!kv || M < 0) return ARIA_Q4_EINVAL;
   if (kv->kv_heads <= 0 || kv->page_size <= 0 || kv->max_pages <= 0 || kv->num_pages < 0 ||
@@ -42,7 +51,8 @@ static int check_kv(const aria_paged_kv* kv, int M, long long* slots) {
   if (kv->page_stride % 8 || kv->slot_stride % 8 || kv->head_stride % 8) return ARIA_Q4_EALIGN;
   if (M == 0) return ARIA_Q4_OK;
   if (!kv->k_pages || !kv->v_pages || !kv->block_table || !kv->lens) return ARIA_Q4_EINVAL;
-  if (!aligned16(kv->k_pages) || !aligned16(kv->v_pages)) return ARIA_Q4_EALIGN;
+  if (!aligned16(kv->k_pages) || !aligned16(kv->v_pages) || !elements_aligned(4, {kv->block_table, kv->lens}))
+    return ARIA_Q4_EALIGN;
   return ARIA_Q4_OK;
 }
 
@@ -86,6 +96,8 @@ int aria_attention_paged(const aria_paged_kv* kv, int M, int heads, const uint16
   if (M == 0) return ARIA_Q4_OK;
   if (!q || !out || !workspace) return ARIA_Q4_EINVAL;
   if (!aligned16(q) || q_row % 8 || q_head % 8) return ARIA_Q4_EALIGN;
+  if (!elements_aligned(2, {out}) || !elements_aligned(4, {lse, weights_in, weights_out, slot_pos, positions}))
+    return ARIA_Q4_EALIGN;
   if (k_new && (!aligned16(k_new) || !aligned16(v_new) || new_row % 8 || new_head % 8)) return ARIA_Q4_EALIGN;
   if (((uintptr_t)workspace & 255u) != 0) return ARIA_Q4_EALIGN;
   if (int s = check_device()) return s;
@@ -139,7 +151,7 @@ int aria_prompt_weights(const uint16_t* q, long long q_seq, long long q_pos, lon
   if (head_dim != 64 && head_dim != 128) return ARIA_Q4_EUNSUPPORTED;
   if (B == 0 || T == 0) return ARIA_Q4_OK;
   if (!q || !k || !lse || !weights) return ARIA_Q4_EINVAL;
-  if (!aligned16(q) || !aligned16(k)) return ARIA_Q4_EALIGN;
+  if (!aligned16(q) || !aligned16(k) || !elements_aligned(4, {lse, weights})) return ARIA_Q4_EALIGN;
   const long long strides[6] = {q_seq, q_pos, q_head, k_seq, k_pos, k_head};
   for (long long s : strides) {
     if (s <= 0) return ARIA_Q4_EINVAL;
@@ -172,6 +184,7 @@ int aria_cache_evict(const aria_paged_kv* kv, int M, const float* weights_in, fl
   if (cap < slots || slots > kEvictMaxSlots) return ARIA_Q4_ESIZE;
   if (M == 0) return ARIA_Q4_OK;
   if (!weights_in || !weights_out || !pos_in || !pos_out || !next_pos || lens_out == kv->lens) return ARIA_Q4_EINVAL;
+  if (!elements_aligned(4, {weights_in, weights_out, pos_in, pos_out, next_pos, lens_out})) return ARIA_Q4_EALIGN;
   if ((long long)M * kv->kv_heads > 0x7fffffffLL / 8) return ARIA_Q4_ESIZE;
   const size_t need = evict_workspace_bytes(M, kv->kv_heads, slots, keep);
   if (need > 0 && !workspace) return ARIA_Q4_EINVAL;
@@ -220,6 +233,11 @@ int aria_logits_adjust(const aria_logit_rules* r, const void* logits, int dtype,
   if (r->allowed_row < 0 || logits_row < 0 || out_row < 0) return ARIA_Q4_EINVAL;
   if (M == 0) return ARIA_Q4_OK;
   if (!logits || !out) return ARIA_Q4_EINVAL;
+  if (!elements_aligned(dtype == ARIA_Q4_F32 ? 4 : 2, {logits}) ||
+      !elements_aligned(out_dtype == ARIA_Q4_F32 ? 4 : 2, {out}) ||
+      !elements_aligned(4, {r->history, r->history_lens, r->prompt_lens, r->repetition, r->frequency, r->presence,
+                            r->bias_tokens, r->bias_values, r->allowed, token}))
+    return ARIA_Q4_EALIGN;
   if (out == logits && (out_dtype != dtype || out_row != logits_row)) return ARIA_Q4_EINVAL;
   if (token) {
     if (!workspace) return ARIA_Q4_EINVAL;

@@ -162,3 +162,38 @@ def test_allowed_mask_words():
     w = allowed_mask(ok)
     assert w.dtype == torch.int32 and w.shape == (2, 3)
     assert w[0].tolist() == [-2**31, 1, 0] and w[1].tolist() == [1, 0, 32]
+
+
+def test_pointers_that_split_an_element_are_refused(lib):
+    """Every kernel reads whole elements: a pointer between two of them never reaches a launch."""
+    from aria_b200._lib import LogitRulesStruct
+
+    def logits(r=None, x=256, dtype=0, out=512, odt=0, tok=None):
+        r = LogitRulesStruct() if r is None else r
+        return lib.aria_logits_adjust(ctypes.byref(r), P(x), dtype, 100, 2, 100, P(out), odt, 100, P(tok), P(256), 99,
+                                      None)
+    assert logits(x=258) == EALIGN and logits(out=514) == EALIGN and logits(x=257, dtype=1, odt=1) == EALIGN
+    assert logits(dtype=1, out=514, odt=0) == EALIGN and logits(tok=258) == EALIGN
+    assert logits(x=258, dtype=1, out=518, odt=1) in (ECUDA, ENODEVICE)
+    for name in ("history", "history_lens", "prompt_lens", "repetition", "frequency", "presence", "bias_tokens",
+                 "bias_values", "allowed"):
+        r = dict(history=256, history_lens=256, history_cap=4, history_row=4, bias_tokens=256, bias_values=256, biases=1)
+        assert logits(LogitRulesStruct(**{**r, name: 258})) == EALIGN, name
+    assert _attend(lib, _kv(lens=258)) == EALIGN and _attend(lib, _kv(block_table=258)) == EALIGN
+    assert _attend(lib, _kv(), out=257) == EALIGN and _attend(lib, _kv(), lse=258) == EALIGN
+    assert _attend(lib, _kv(), wi=258, wo=256) == EALIGN and _attend(lib, _kv(), wi=256, wo=258) == EALIGN
+    new = dict(wi=256, wo=256, kn=256, vn=256)
+    assert _attend(lib, _kv(), sp=258, pos=256, **new) == EALIGN
+    assert _attend(lib, _kv(), sp=256, pos=258, **new) == EALIGN
+
+    def evict(**kw):
+        a = {**dict(wi=256, wo=256, pi=256, po=256, nxt=256, lo=None), **kw}
+        return lib.aria_cache_evict(ctypes.byref(_kv()), 1, P(a["wi"]), P(a["wo"]), P(a["pi"]), P(a["po"]), 64,
+                                    P(a["nxt"]), 32, 0, 0, P(a["lo"]), P(256), 1 << 20, None)
+    for name in ("wi", "wo", "pi", "po", "nxt", "lo"):
+        assert evict(**{name: 258}) == EALIGN, name
+
+    def prompt(lse=256, w=256):
+        return lib.aria_prompt_weights(P(256), 64, 64, 64, P(256), 64, 64, 64, 1, 1, 8, 2, 1, 64, P(lse), 0.1, 0, P(w),
+                                       8, 8, None, 0, None)
+    assert prompt(lse=258) == EALIGN and prompt(w=258) == EALIGN and prompt() in (ECUDA, ENODEVICE)
