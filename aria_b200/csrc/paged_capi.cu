@@ -56,6 +56,12 @@ static int check_kv(const aria_paged_kv* kv, int M, long long* slots) {
   return ARIA_Q4_OK;
 }
 
+// the key blocks of all sequences and heads, and the query blocks of a key block, count in 31 bits
+static bool prompt_blocks_fit(int B, int T, int heads, int kv_heads) {
+  const long long blocks = ((long long)T + 127) / 128, most = 0x7fffffffLL / 1024;
+  return blocks <= most / kv_heads / B && blocks <= 0x7fffffffLL / heads;
+}
+
 extern "C" {
 
 size_t aria_paged_workspace_counter_bytes(void) {
@@ -137,7 +143,9 @@ int aria_attention_paged(const aria_paged_kv* kv, int M, int heads, const uint16
 }
 
 size_t aria_prompt_weights_workspace_bytes(int B, int T, int heads, int kv_heads, int first_query) {
-  if (B <= 0 || T <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || first_query < 0) return 0;
+  if (B <= 0 || T <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || first_query < 0 ||
+      !prompt_blocks_fit(B, T, heads, kv_heads))
+    return 0;
   return prompt_workspace_bytes(B, T, kv_heads, heads / kv_heads, first_query);
 }
 
@@ -158,7 +166,7 @@ int aria_prompt_weights(const uint16_t* q, long long q_seq, long long q_pos, lon
     if (s % 8) return ARIA_Q4_EALIGN;
     if (s >= (1LL << 38)) return ARIA_Q4_ESIZE;  // the tensor maps' strides are 40 bits of bytes
   }
-  if ((long long)B * kv_heads * ((T + 127) / 128) > 0x7fffffffLL / 1024) return ARIA_Q4_ESIZE;
+  if (!prompt_blocks_fit(B, T, heads, kv_heads)) return ARIA_Q4_ESIZE;
   if (((uintptr_t)workspace & 255u) != 0) return ARIA_Q4_EALIGN;
   if (int s = check_device()) return s;
   const size_t need = prompt_workspace_bytes(B, T, kv_heads, heads / kv_heads, first_query);
@@ -231,6 +239,9 @@ int aria_logits_adjust(const aria_logit_rules* r, const void* logits, int dtype,
   if (r->history && (!r->history_lens || r->history_cap < 0)) return ARIA_Q4_EINVAL;
   if (r->bias_tokens && (!r->bias_values || r->biases < 0)) return ARIA_Q4_EINVAL;
   if (r->allowed_row < 0 || logits_row < 0 || out_row < 0) return ARIA_Q4_EINVAL;
+  // indexes run in 31 bits, up to a chunk and a block's step past the last one
+  const int most = 0x7fffffff - (1 << 16);
+  if (V > most || r->history_cap > most || r->biases > most) return ARIA_Q4_ESIZE;
   if (M == 0) return ARIA_Q4_OK;
   if (!logits || !out) return ARIA_Q4_EINVAL;
   if (!elements_aligned(dtype == ARIA_Q4_F32 ? 4 : 2, {logits}) ||

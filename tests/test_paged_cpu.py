@@ -197,3 +197,24 @@ def test_pointers_that_split_an_element_are_refused(lib):
         return lib.aria_prompt_weights(P(256), 64, 64, 64, P(256), 64, 64, 64, 1, 1, 8, 2, 1, 64, P(lse), 0.1, 0, P(w),
                                        8, 8, None, 0, None)
     assert prompt(lse=258) == EALIGN and prompt(w=258) == EALIGN and prompt() in (ECUDA, ENODEVICE)
+
+
+def test_sizes_past_31_bits_are_refused(lib):
+    """Sizes near 2^31, where the kernels' block counts and steps would wrap."""
+    from aria_b200._lib import LogitRulesStruct
+    top = 2**31 - 1
+
+    def prompt(B, T, kvh=1, heads=None):
+        return lib.aria_prompt_weights(P(256), 64, 64, 64, P(256), 64, 64, 64, 1, B, T, heads or kvh, kvh, 64, P(256),
+                                       0.1, 0, P(256), 8, 8, None, 0, None)
+    for T in (top, top - 126, 2**28 + 1):
+        assert prompt(1, T) == ESIZE and lib.aria_prompt_weights_workspace_bytes(1, T, 1, 1, 0) == 0
+    assert prompt(2**16, 2**13) == ESIZE and prompt(1, 2**20, heads=2**18 + 1) == ESIZE
+    assert prompt(1, 2**28 - 128) in (ECUDA, ENODEVICE)
+
+    def logits(V=100, **kw):
+        r = LogitRulesStruct(**kw)
+        return lib.aria_logits_adjust(ctypes.byref(r), P(256), 1, 8, 1, V, P(256), 1, 8, None, None, 0, None)
+    assert logits(V=top) == ESIZE and logits(V=2**31 - 2**17) in (ECUDA, ENODEVICE)
+    assert logits(history=256, history_lens=256, history_cap=top) == ESIZE
+    assert logits(bias_tokens=256, bias_values=256, biases=top) == ESIZE
