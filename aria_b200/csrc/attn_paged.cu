@@ -20,6 +20,10 @@
 //  * each warp streams its own tiles through a cp.async ring in shared memory,
 //    several tiles ahead and across pair boundaries, so loads never wait for
 //    arithmetic;
+//  * a maximum passes NaN over, a sum does not: a row's sum is 0 exactly when nothing
+//    was there to attend over, and NaN when a score was NaN or +inf.  So the sum
+//    alone says whether a state is empty, and NaN reaches out, lse and the weights
+//    whichever way a pair is cut;
 //  * both products run on warp-level tensor-core MMAs (m16n8k16): rows of A are
 //    the query heads.  With at most 8 of them per MMA the other 8 rows carry, in
 //    P V, the part of P that rounding to 16 bits drops (p = hi + lo), so the
@@ -194,7 +198,7 @@ __device__ __noinline__ void paged_join(const PagedArgs& a, const PagedCut cut, 
       float w = cnt <= 32 ? paged_ex2(mx - ms) : 0.0f;  // up to 32 states: lane k's maximum is state k's
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       float acc[VEC];
 #pragma unroll
       for (int v = 0; v < VEC; v++) acc[v] = 0.0f;
@@ -621,7 +625,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
         const int h = g + 8 * rb;
         if (h >= rows) continue;
         if (all) {
-          const float inv = l[rb] > 0.0f ? 1.0f / l[rb] : 0.0f;
+          const float inv = l[rb] == 0.0f ? 0.0f : 1.0f / l[rb];
 #pragma unroll
           for (int j = 0; j < DH / 8; j++) {
             paged_store<BF16>(a, seg.m, h0 + h, 8 * j + 2 * t4, (o[rb][j][0] + o[rb][j][2]) * inv);
@@ -690,13 +694,14 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
     float acc = 0.0f, l = 0.0f;
 #pragma unroll
     for (int w = 0; w < kPagedWarps; w++) {
+      const float lw = st[w][srows * DH + srows + h];
+      if (lw == 0.0f) continue;  // an empty state's O was not written
       const float x = paged_ex2(st[w][srows * DH + h] - ms);
-      if (x == 0.0f) continue;  // an empty state's O was not written
       acc = fmaf(x, st[w][e], acc);
-      l = fmaf(x, st[w][srows * DH + srows + h], l);
+      l = fmaf(x, lw, l);
     }
     if (alone) {
-      paged_store<BF16>(a, pair0.m, h0 + h, e % DH, l > 0.0f ? acc / l : 0.0f);
+      paged_store<BF16>(a, pair0.m, h0 + h, e % DH, l == 0.0f ? 0.0f : acc / l);
       if (e % DH == 0) paged_store_lse<WEIGHTS>(a, pair0.m, h0 + h, m, l);
     } else {
       part[e] = acc;

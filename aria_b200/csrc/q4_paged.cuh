@@ -107,10 +107,10 @@ __device__ __forceinline__ void paged_store(const PagedArgs& a, int m, int h, in
     reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(v);
 }
 
-// mx: the row's maximum in the log2 domain, sum: of 2^(s - mx)
+// mx: the row's maximum in the log2 domain, sum: of 2^(s - mx), 0 for a row that saw nothing
 template <bool WEIGHTS>
 __device__ __forceinline__ void paged_store_lse(const PagedArgs& a, int m, int h, float mx, float sum) {
-  const float l2 = sum > 0.0f ? mx + log2f(sum) : -INFINITY;
+  const float l2 = sum == 0.0f ? -INFINITY : mx + log2f(sum);
   if (a.lse) a.lse[(size_t)m * a.Hq + h] = l2 * 0.69314718055994531f;
   if (WEIGHTS) a.lse2[(size_t)m * a.Hq + h] = l2;
 }

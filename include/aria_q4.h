@@ -307,7 +307,9 @@ typedef struct {
  *     out[m][h] = sum_j p_j v_j,  p_j = exp(scale q.k_j - lse[m][h])
  * lse [M][heads] (natural log; may be NULL) = ln sum_j exp(scale q.k_j).  A sequence
  * without slots (n = 0, every page absent, or no room left for the new token) gives
- * zeros and -inf.  Softmax and sums in f32; p enters the product with V as the sum
+ * zeros and -inf.  A score of -inf weighs nothing; one of NaN or +inf makes that head's
+ * out and lse NaN, and the group's weights; a value that is NaN or infinite makes its
+ * component of out NaN or infinite.  Softmax and sums in f32; p enters the product with V as the sum
  * of two 16-bit values.
  * weights_in, weights_out (f32 [M][kv_heads][weights_cap >= max_pages page_size];
  * both or neither; may be one buffer): for j < n

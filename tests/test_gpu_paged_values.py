@@ -1,0 +1,78 @@
+"""The paged attention on values that a model should not produce but may: NaN, infinities, and
+scores far apart.  Every case is compared with the 64-bit restatement at lengths that take
+each way through the kernel: one CTA per pair (short, few), joined states (long), pairs
+that one warp finishes (short, many)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged_np
+
+pytestmark = [pytest.mark.gpu,
+              pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
+
+# of p, lse and weights: as derived in test_gpu_paged.py
+REL_P = 3e-5
+ROUND = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+WAYS = [(40, 1), (500, 1), (5000, 1), (40, 300), (700, 40)]
+
+
+def _f64(t):
+    return t.detach().float().cpu().numpy().astype(np.float64)
+
+
+def _cache(n, M, H, dh, dtype, seed):
+    """M sequences of n slots in pages of 16, in order."""
+    from aria_b200.paged import PagedKV
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    per = -(-n // 16)
+    k, v = (torch.randn(M * per, 16, H, dh, generator=g, device="cuda").to(dtype) for _ in range(2))
+    table = torch.arange(M * per, dtype=torch.int32, device="cuda").view(M, per)
+    kv = PagedKV(k, v, table, torch.full((M,), n, dtype=torch.int32, device="cuda"))
+    q = torch.randn(M, 2 * H, dh, generator=g, device="cuda").to(dtype)
+    return kv, q, k.view(M, per * 16, H, dh)[:, :n], v.view(M, per * 16, H, dh)[:, :n]
+
+
+@pytest.mark.parametrize("n,M", WAYS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("what", ["q nan", "key nan", "key inf", "key -inf", "keys -inf", "value nan", "value inf"])
+def test_nan_and_infinities_reach_the_outputs(what, dtype, n, M):
+    from aria_b200.paged import attention_paged
+    H, dh, m, at = 2, 64, M // 2, n // 3
+    kv, q, k, v = _cache(n, M, H, dh, dtype, n + M)
+    q[m, :, 5] = torch.tensor([0.5, -0.5, 0.5, 0.5])  # (the sign that an infinite key component meets)
+    if what == "q nan":
+        q[m, 1, 7] = float("nan")
+    elif what == "key nan":
+        k[m, at, 0, 7] = float("nan")
+    elif what in ("key inf", "key -inf"):
+        k[m, at, 0, 5] = float(what[4:])
+    elif what == "keys -inf":  # nothing left for head 0, everything +inf for head 1
+        k[m, :, 0, 5] = -float("inf")
+    elif what == "value nan":
+        v[m, at, 0, 9] = float("nan")
+    else:
+        v[m, at, 0, 9] = float("inf")
+    w = torch.zeros(M, H, kv.slots, device="cuda")
+    out, lse = attention_paged(q, kv, want_lse=True, weights=w)
+    for i in {0, m, M - 1}:
+        with np.errstate(invalid="ignore"):
+            ro, rl, rp = paged_np.attend(_f64(q[i]), _f64(k[i]), _f64(v[i]), 1 / math.sqrt(dh))
+        rw = rp.reshape(H, 2, n).sum(1)
+        o, l, ww = _f64(out[i]), _f64(lse[i]), _f64(w[i, :, :n])
+        if i == m and what == "keys -inf":  # as an empty row; the weights are head 1's
+            assert np.all(o[0] == 0) and l[0] == -np.inf
+            ro[0], rl[0] = 0, -np.inf
+        if i == m and what.startswith("value"):  # one component of the group's two heads
+            assert not np.isfinite(o[:2, 9]).any()
+            o[:2, 9], ro[:2, 9] = 0, 0
+        assert np.array_equal(np.isnan(o), np.isnan(ro)), (what, i)
+        assert np.array_equal(np.isnan(l), np.isnan(rl)) and np.array_equal(np.isnan(ww), np.isnan(rw))
+        bad = np.isnan(ro)
+        assert np.all((np.abs(o - ro) <= ROUND[dtype] * np.abs(ro) + REL_P * 6)[~bad])
+        bad = np.isnan(rl) | np.isinf(rl)
+        assert np.array_equal(l[np.isinf(rl)], rl[np.isinf(rl)]) and np.all((np.abs(l - rl) <= REL_P)[~bad])
+        bad = np.isnan(rw)
+        assert np.all((np.abs(ww - rw) <= REL_P * rw + 1e-6)[~bad])
