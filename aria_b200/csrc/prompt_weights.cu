@@ -135,7 +135,8 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // (n from the low bits of x + 1.5 2^23), a polynomial in f of degree 5 whose coefficients
 // minimise the largest relative error on that interval (Lawson's iteration; 2.3e-7
 // evaluated in f32), and n added to the exponent.  x below -126 gives 0 (-inf does, for
-// masked queries), x above 127 gives 2^127, NaN stays NaN.
+// masked queries), x above 127 gives 2^127.  NaN stays NaN: it goes round the addition to
+// the exponent, which would make a large finite number of its bits.
 __device__ __forceinline__ uint64_t both(float x) { return pack2(__float_as_uint(x), __float_as_uint(x)); }
 __device__ __forceinline__ void exp2_poly2(float& x, float& y) {
   asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(127.0f));
@@ -151,8 +152,11 @@ __device__ __forceinline__ void exp2_poly2(float& x, float& y) {
   float p0, p1, t0, t1;
   unpack2(p, p0, p1);
   unpack2(t, t0, t1);
-  x = x < -126.0f ? 0.0f : __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23));
-  y = y < -126.0f ? 0.0f : __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23));
+  float x0, y0;  // 0, or the NaN
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(x), "f"(0.0f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y0) : "f"(y), "f"(0.0f));
+  x = x >= -126.0f ? __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23)) : x0;
+  y = y >= -126.0f ? __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23)) : y0;
 }
 
 template <int DH, bool BF16>

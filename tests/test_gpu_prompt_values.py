@@ -1,0 +1,31 @@
+"""Prompt weights on values that a model should not produce but may, against the 64-bit
+restatement.  Tolerance: as derived in test_gpu_paged.py (terms right to 3e-5)."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged_np
+
+pytestmark = [pytest.mark.gpu,
+              pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
+
+
+def _f64(t):
+    return t.detach().float().cpu().numpy().astype(np.float64)
+
+
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("residue", range(16))
+def test_a_nan_query_makes_the_weights_of_its_keys_nan(residue, dh):
+    """At every position of 16 queries (their exponentials are computed in two ways), in a block that
+    the mask cuts and in ones that it does not: NaN for keys up to the query, sound past it."""
+    from aria_b200.paged import prompt_weights
+    g = torch.Generator(device="cuda").manual_seed(residue)
+    T, t = 600, 416 + residue
+    q, k = (torch.randn(1, T, 1, dh, generator=g, device="cuda").half() for _ in range(2))
+    _, rows = paged_np.prompt_weights(_f64(q[0]), _f64(k[0]), dh ** -0.5)
+    ref, _ = paged_np.prompt_weights(_f64(q[0]), _f64(k[0]), dh ** -0.5, t + 1, rows)
+    q[0, t, 0, 3] = float("nan")
+    got = _f64(prompt_weights(q, k, torch.from_numpy(rows)[None].float().cuda())[0, 0])
+    assert np.isnan(got[:t + 1]).all()
+    assert np.all(np.abs(got[t + 1:] - ref[0, t + 1:]) <= 5e-5 * ref[0, t + 1:] + 1e-6)
