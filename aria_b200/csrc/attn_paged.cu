@@ -26,9 +26,12 @@
 //    whichever way a pair is cut;
 //  * both products run on warp-level tensor-core MMAs (m16n8k16): rows of A are
 //    the query heads.  With at most 8 of them per MMA the other 8 rows carry, in
-//    P V, the part of P that rounding to 16 bits drops (p = hi + lo), so the
-//    weights of V are exact to ~2^-17 (f16 to 2^-22) at no cost.  tcgen05 has
-//    nothing to give here: its 128-row tiles would be 1/128 used at G = 1.
+//    P V, the part of P that rounding to 16 bits drops (p = hi + lo).  bf16 holds
+//    the weights of V to 2^-17 of themselves; f16, whose smallest step is 2^-24,
+//    holds 2^15 p, so the weights are right to 2^-22 of themselves or 2^-40 of the
+//    largest, whichever is more (unscaled, a slot 17 behind the leading one was
+//    lost, and with it all of 32749 such slots).  tcgen05 has nothing to give here:
+//    its 128-row tiles would be 1/128 used at G = 1.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -66,6 +69,13 @@ __device__ __forceinline__ void paged_mma(float (&d)[4], uint32_t a0, uint32_t a
   else
     mma_16816(d, a0, a1, a2, a3, b0, b1);
 }
+
+// What p (at most 1) is multiplied by for the product with V, and its inverse: powers
+// of two, so both are exact.
+template <bool BF16>
+struct PagedP {
+  static constexpr float kUp = BF16 ? 1.0f : 32768.0f, kDown = 1.0f / kUp;
+};
 
 // (x, y) rounded to the 16-bit type, and the pair of what the rounding dropped
 template <bool BF16>
@@ -585,7 +595,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
           for (int j = 0; j < TS / 8; j++) {
             const float p0 = paged_ex2(s[j][2 * rb] - msub), p1 = paged_ex2(s[j][2 * rb + 1] - msub);
             l[rb] += p0 + p1;
-            split_pair<BF16>(p0, p1, ph[rb][j], pl[rb][j]);
+            split_pair<BF16>(p0 * PagedP<BF16>::kUp, p1 * PagedP<BF16>::kUp, ph[rb][j], pl[rb][j]);
           }
         }
 
@@ -625,7 +635,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
         const int h = g + 8 * rb;
         if (h >= rows) continue;
         if (all) {
-          const float inv = l[rb] == 0.0f ? 0.0f : 1.0f / l[rb];
+          const float inv = l[rb] == 0.0f ? 0.0f : PagedP<BF16>::kDown / l[rb];
 #pragma unroll
           for (int j = 0; j < DH / 8; j++) {
             paged_store<BF16>(a, seg.m, h0 + h, 8 * j + 2 * t4, (o[rb][j][0] + o[rb][j][2]) * inv);
@@ -636,7 +646,8 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
 #pragma unroll
           for (int j = 0; j < DH / 8; j++)
             *reinterpret_cast<float2*>(state + h * DH + 8 * j + 2 * t4) =
-                make_float2(o[rb][j][0] + o[rb][j][2], o[rb][j][1] + o[rb][j][3]);
+                make_float2((o[rb][j][0] + o[rb][j][2]) * PagedP<BF16>::kDown,
+                            (o[rb][j][1] + o[rb][j][3]) * PagedP<BF16>::kDown);
           if (t4 == 0) {
             state[srows * DH + h] = mx[rb];
             state[srows * DH + srows + h] = l[rb];

@@ -76,3 +76,37 @@ def test_nan_and_infinities_reach_the_outputs(what, dtype, n, M):
         assert np.array_equal(l[np.isinf(rl)], rl[np.isinf(rl)]) and np.all((np.abs(l - rl) <= REL_P)[~bad])
         bad = np.isnan(rw)
         assert np.all((np.abs(ww - rw) <= REL_P * rw + 1e-6)[~bad])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lead", [10.0, 17.0, 17.5, 20.0, 24.0])
+def test_many_small_weights_beside_one_that_leads(lead, dtype):
+    """One slot (an attention sink) leads by `lead` over 32749 others; its value is 0, theirs 1: the
+    output is the others' share alone.  More pairs than warps, so that each pair is one warp's.
+    Weights are right to 3e-5 of themselves or (f16) 2^-40 of the largest; the output is rounded
+    once, to at best 2^-25 (f16)."""
+    from aria_b200.paged import PagedKV, attention_paged
+    M, H, dh, n, ps = 64, 20, 32, 32750, 50
+    k, v = torch.zeros(n // ps, ps, H, dh, dtype=dtype, device="cuda"), torch.ones(n // ps, ps, H, dh, dtype=dtype,
+                                                                                  device="cuda")
+    k[0, 5, :, 0] = lead
+    v[0, 5] = 0
+    table = torch.arange(n // ps, dtype=torch.int32, device="cuda").expand(M, -1).contiguous()  # one cache for all
+    q = torch.zeros(M, H, dh, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1
+    kv = PagedKV(k, v, table, torch.full((M,), n, dtype=torch.int32, device="cuda"))
+    out, _ = attention_paged(q, kv, scale=1.0)
+    share = (n - 1) * math.exp(-lead) / (1 + (n - 1) * math.exp(-lead))
+    tol = (ROUND[dtype] + 3e-5) * share + (n * 2.0 ** -40 + 2.0 ** -25 if dtype is torch.float16 else 0)
+    assert np.abs(_f64(out) - share).max() <= tol
+
+
+def test_large_values_with_many_equal_weights():
+    """The largest f16 value in every slot: scaled weights times it, summed over 40000 slots."""
+    from aria_b200.paged import PagedKV, attention_paged
+    n, H, dh = 40000, 2, 64
+    k, v = (torch.full((n // 16, 16, H, dh), x, dtype=torch.float16, device="cuda") for x in (0.0, 65504.0))
+    table = torch.arange(n // 16, dtype=torch.int32, device="cuda").view(1, -1)
+    kv = PagedKV(k, v, table, torch.tensor([n], dtype=torch.int32, device="cuda"))
+    out, _ = attention_paged(torch.ones(1, H, dh, dtype=torch.float16, device="cuda"), kv)
+    assert bool((out == 65504.0).all())
