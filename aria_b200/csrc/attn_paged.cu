@@ -495,11 +495,13 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
         }
       }
       float o[RB][DH / 8][4];
-      float mx[RB], l[RB];
+      // maximum and sum; l_off: what rounding has put too much into the sum, taken out of
+      // the next tile's (small weights after a large one would otherwise not count)
+      float mx[RB], l[RB], l_off[RB];
 #pragma unroll
       for (int rb = 0; rb < RB; rb++) {
         mx[rb] = -INFINITY;
-        l[rb] = 0.0f;
+        l[rb] = l_off[rb] = 0.0f;
 #pragma unroll
         for (int j = 0; j < DH / 8; j++)
 #pragma unroll
@@ -585,18 +587,23 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
           if (__any_sync(0xffffffffu, m_new > mx[rb])) {
             const float alpha = paged_ex2(mx[rb] - msub);
             l[rb] *= alpha;
+            l_off[rb] *= alpha;
 #pragma unroll
             for (int j = 0; j < DH / 8; j++)
 #pragma unroll
               for (int e = 0; e < 4; e++) o[rb][j][e] *= alpha;
             mx[rb] = m_new;
           }
+          float sum = -l_off[rb];
 #pragma unroll
           for (int j = 0; j < TS / 8; j++) {
             const float p0 = paged_ex2(s[j][2 * rb] - msub), p1 = paged_ex2(s[j][2 * rb + 1] - msub);
-            l[rb] += p0 + p1;
+            sum += p0 + p1;
             split_pair<BF16>(p0 * PagedP<BF16>::kUp, p1 * PagedP<BF16>::kUp, ph[rb][j], pl[rb][j]);
           }
+          const float l_new = l[rb] + sum;
+          l_off[rb] = (l_new - l[rb]) - sum;
+          l[rb] = l_new;
         }
 
         // O += P V: rows 0-7 the rounded weights, rows 8-15 what the rounding dropped

@@ -110,3 +110,20 @@ def test_large_values_with_many_equal_weights():
     kv = PagedKV(k, v, table, torch.tensor([n], dtype=torch.int32, device="cuda"))
     out, _ = attention_paged(torch.ones(1, H, dh, dtype=torch.float16, device="cuda"), kv)
     assert bool((out == 65504.0).all())
+
+
+@pytest.mark.parametrize("lead", [0.0, 10.0, 17.0, 17.5, 20.0])
+@pytest.mark.parametrize("at", [5, 20000])
+def test_log_sum_exp_of_many_small_weights_beside_one_that_leads(at, lead):
+    """The sum of 32749 weights of exp(-lead) and one of 1, in one warp's running sum; lse is right
+    to 3e-5 as everywhere, whatever comes first."""
+    from aria_b200.paged import PagedKV, attention_paged
+    M, H, dh, n, ps = 64, 20, 32, 32750, 50
+    k, v = (torch.zeros(n // ps, ps, H, dh, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    k[at // ps, at % ps, :, 0] = lead
+    table = torch.arange(n // ps, dtype=torch.int32, device="cuda").expand(M, -1).contiguous()
+    q = torch.zeros(M, H, dh, dtype=torch.bfloat16, device="cuda")
+    q[:, :, 0] = 1
+    kv = PagedKV(k, v, table, torch.full((M,), n, dtype=torch.int32, device="cuda"))
+    _, lse = attention_paged(q, kv, scale=1.0, want_lse=True)
+    assert np.abs(_f64(lse) - lead - math.log1p((n - 1) * math.exp(-lead))).max() <= REL_P
