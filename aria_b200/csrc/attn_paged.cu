@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
         const int hk = a.chunks == 1 ? pf.hv : pf.hv / a.chunks;
         const int slot0 = pf.tile * TS, have = slots[pf.m] - slot0;  // slots of the pair from here on
         const uint32_t dst = ring_s + st * C::kStageBytes;
-        const int last = a.k_new != nullptr && have <= TS ? have - 1 : TS;  // row of the new token, if here
+        int last = a.k_new != nullptr && have <= TS ? have - 1 : TS;  // row of the new token, if here
         const long long noff = (long long)pf.m * a.new_row + (long long)hk * a.new_head;
         uint32_t valid;
         if (PAGE16) {
@@ -419,7 +419,9 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
               }
             }
           } else {
-            if (last < TS) valid |= 1u << last;
+            // (valid has the new token's bit where its page exists; elsewhere its slot is absent
+            // like any other)
+            if (last < TS && !((valid >> last) & 1u)) last = TS;
 #pragma unroll
             for (int i = 0; i < TS * CPR / 32; i++) {
               const int rh = RPI * i;  // first row of this copy; all of one half
@@ -439,7 +441,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) attn_paged_kernel(const __gr
         } else {
           const int slot = slot0 + lane;
           long long off = -1;  // element offset of this lane's row in the pages
-          if (lane == last)
+          if (page >= 0 && lane == last)
             off = -2;
           else if (page >= 0)
             off = (long long)page * a.page_stride + (long long)(slot - page_index(slot) * a.page_size) * a.slot_stride +

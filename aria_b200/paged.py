@@ -169,7 +169,8 @@ def attention_paged(q: torch.Tensor, kv: PagedKV, *, k_new: torch.Tensor | None 
                     positions: torch.Tensor | None = None):
     """q [M][heads][head_dim] (any strides that are multiples of 8): one new token per
     sequence.  k_new, v_new [M][kv_heads][head_dim]: its own rows, stored at slot
-    lens[m] and part of the attention (lens is the caller's to advance).  Returns (out
+    lens[m] and part of the attention (lens is the caller's to advance); where the table
+    has no page for that slot they are neither.  Returns (out
     [M][heads][head_dim], lse f32 [M][heads] or None); a sequence without slots gives
     zeros and -inf.  scale defaults to 1 / sqrt(head_dim).
 

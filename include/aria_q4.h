@@ -302,7 +302,9 @@ typedef struct {
  * dtype (element strides q_row, q_head); heads a multiple of kv_heads, query head h
  * reading key/value head h / (heads / kv_heads).  With k_new, v_new ([M][kv_heads]
  * [head_dim]; both or neither) the new token's rows are stored at slot lens[m] and
- * take part; lens itself is the caller's to advance.  Over the n slots (lens[m], + 1
+ * take part; lens itself is the caller's to advance.  Where that slot has no page it is
+ * absent like any other: the token's rows are stored nowhere and take no part, its weight
+ * is 0 (its position is listed all the same).  Over the n slots (lens[m], + 1
  * with k_new):
  *     out[m][h] = sum_j p_j v_j,  p_j = exp(scale q.k_j - lse[m][h])
  * lse [M][heads] (natural log; may be NULL) = ln sum_j exp(scale q.k_j).  A sequence

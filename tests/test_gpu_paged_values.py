@@ -127,3 +127,44 @@ def test_log_sum_exp_of_many_small_weights_beside_one_that_leads(at, lead):
     kv = PagedKV(k, v, table, torch.full((M,), n, dtype=torch.int32, device="cuda"))
     _, lse = attention_paged(q, kv, scale=1.0, want_lse=True)
     assert np.abs(_f64(lse) - lead - math.log1p((n - 1) * math.exp(-lead))).max() <= REL_P
+
+
+@pytest.mark.parametrize("ps,dh", [(16, 64), (48, 64), (16, 128), (24, 64), (5, 128), (7, 256)])
+@pytest.mark.parametrize("n", [0, 95, 96, 111, 240, 700])
+def test_a_new_token_whose_page_is_absent(n, ps, dh):
+    """Its slot is absent like any other: not stored, no part in the attention, weight 0, its position
+    listed.  A second sequence, whose page is there, is not affected."""
+    from aria_b200.paged import PagedKV, attention_paged
+    H, M = 2, 2
+    g = torch.Generator(device="cuda").manual_seed(n + ps)
+    per = n // ps + 2
+    k, v = (torch.randn(M * per, ps, H, dh, generator=g, device="cuda").half() for _ in range(2))
+    table = torch.arange(M * per, dtype=torch.int32, device="cuda").view(M, per)
+    table[0, n // ps] = -1
+    kv = PagedKV(k, v, table, torch.full((M,), n, dtype=torch.int32, device="cuda"))
+    q = torch.randn(M, H, dh, generator=g, device="cuda").half()
+    kn, vn = (torch.randn(M, H, dh, generator=g, device="cuda").half() for _ in range(2))
+    w = torch.rand(M, H, kv.slots, generator=g, device="cuda")
+    pos = torch.full((M, H, kv.slots), -7, dtype=torch.int32, device="cuda")
+    k0, v0, w0 = k.clone(), v.clone(), w.clone()
+    out, lse = attention_paged(q, kv, k_new=kn, v_new=vn, want_lse=True, weights=w, slot_pos=pos,
+                               positions=torch.tensor([50, 51], dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+    at = 1 * per + n // ps
+    assert torch.equal(k[at, n % ps], kn[1]) and torch.equal(v[at, n % ps], vn[1])
+    k[at, n % ps], v[at, n % ps] = k0[at, n % ps], v0[at, n % ps]
+    assert torch.equal(k, k0) and torch.equal(v, v0)
+    for m in range(M):
+        keys, vals = (torch.cat([x.view(M, per * ps, H, dh)[m, :n], new[m:m + 1]]) for x, new in ((k0, kn), (v0, vn)))
+        present = np.ones(n + 1, dtype=bool)
+        if m == 0:
+            present[n // ps * ps:] = False
+        ro, rl, rp = paged_np.attend(_f64(q[m]), _f64(keys), _f64(vals), dh ** -0.5, present)
+        assert np.all(np.abs(_f64(out[m]) - ro) <= ROUND[torch.float16] * np.abs(ro) + REL_P * 6), m
+        l = _f64(lse[m])
+        assert np.array_equal(np.isinf(l), np.isinf(rl)) and np.all(np.abs(l - rl)[~np.isinf(rl)] <= REL_P)
+        want = rp.copy()
+        want[:, :n] += _f64(w0[m, :, :n])
+        assert np.all(np.abs(_f64(w[m, :, :n + 1]) - want) <= REL_P * want + 1e-6)
+        assert m == 1 or bool((w[0, :, n] == 0).all())
+        assert bool((pos[m, :, n] == 50 + m).all()) and bool((pos[m, :, :n] == -7).all())
