@@ -134,7 +134,7 @@ def fastcall():
         from . import _fastcall
         lib = _lib()
         _fastcall.bind(*(ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
-            "aria_attention_paged", "aria_prompt_weights", "aria_cache_evict", "aria_logits_adjust")))
+            "aria_attention_paged", "aria_prompt_weights", "aria_cache_evict", "aria_logits_adjust")), check)
         _FAST = _fastcall
     return _FAST
 

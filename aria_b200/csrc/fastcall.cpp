@@ -6,13 +6,17 @@
 // checks of aria_b200/paged.py and logits.py are made in C++ and the C ABI is called
 // directly (attention of one sequence: 4.7 us of host time per call instead of 11.9,
 // most of it the launch and the lse's allocation; logits of one row: 6.5 instead of 16).
-// A function returns None when anything is unusual -- an argument that does not pass, a
-// workspace that has to grow, a status other than 0 -- and the Python code then goes the
-// long way, which says what is wrong.  No arithmetic and no CUDA call happens here.
+// A function returns None when anything is unusual and nothing was launched -- an argument
+// that does not pass, a workspace that has to grow, a call that the library refuses -- and
+// the Python code then goes the long way, which says what is wrong.  A CUDA error raises
+// here: one of a call's kernels may have run, and sums, moves and stored rows are not to
+// be made twice.  No arithmetic and no CUDA call happens here.
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+
+#include <exception>
 
 #include "../../include/aria_q4.h"
 
@@ -22,6 +26,26 @@ decltype(&aria_attention_paged) f_attention = nullptr;
 decltype(&aria_prompt_weights) f_prompt = nullptr;
 decltype(&aria_cache_evict) f_evict = nullptr;
 decltype(&aria_logits_adjust) f_logits = nullptr;
+
+PyObject* check = nullptr;  // _lib.check(name, status): raises what the status means
+
+thread_local bool launched = false;  // the library was called, and did not refuse
+
+// Whether the library refused the call, so that the long way may make it again.  `failed`:
+// it did not, and an exception is set.
+bool refused(const char* name, int status, bool& failed) {
+  failed = false;
+  if (status == ARIA_Q4_OK) return false;
+  if (status != ARIA_Q4_ECUDA) {
+    launched = false;
+    return true;
+  }
+  failed = true;
+  PyObject* r = PyObject_CallFunction(check, "si", name, status);
+  Py_XDECREF(r);
+  if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, name);
+  return false;
+}
 
 struct Args {
   PyObject* const* a;
@@ -117,11 +141,14 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   if (!rows(*out, type, dev, M, heads, dh, orow, oh)) Py_RETURN_NONE;
   if (want_lse) lse = at::empty({M, heads}, q->options().dtype(at::kFloat));
+  launched = true;
   const int status = f_attention(
       kv, M, (int)heads, ptr<const uint16_t>(q), qr, qh, ptr<const uint16_t>(kn), ptr<const uint16_t>(vn), nr, nh, scale,
       ptr<uint16_t>(out), orow, oh, want_lse ? ptr<float>(&lse) : nullptr, ptr<const float>(w),
       wo ? ptr<float>(wo) : ptr<float>(w), cap, ptr<int>(sp), sp ? ptr<const int>(pos) : nullptr, ws, ws_bytes, stream);
-  if (status != ARIA_Q4_OK) Py_RETURN_NONE;
+  bool failed;
+  if (refused("aria_attention_paged", status, failed)) Py_RETURN_NONE;
+  if (failed) return nullptr;
   PyObject* r = PyTuple_New(2);
   if (!r) return nullptr;
   if (made.defined()) {
@@ -164,11 +191,14 @@ PyObject* prompt(PyObject*, PyObject* const* args, Py_ssize_t n) {
       out->size(1) != kvh || out->size(2) < T || (out->stride(2) != 1 && out->size(2) > 1))
     Py_RETURN_NONE;
   auto st = [](const at::Tensor* t, int d) { return t->size(d) > 1 ? (long long)t->stride(d) : 8LL; };
+  launched = true;
   const int status =
       f_prompt(ptr<const uint16_t>(q), st(q, 0), st(q, 1), st(q, 2), ptr<const uint16_t>(k), st(k, 0), st(k, 1), st(k, 2),
                type_code(type), (int)B, (int)T, (int)heads, (int)kvh, (int)dh, ptr<const float>(lse), scale, (int)first,
                ptr<float>(out), out->stride(0), out->stride(1), ws, ws_bytes, stream);
-  if (status != ARIA_Q4_OK) Py_RETURN_NONE;
+  bool failed;
+  if (refused("aria_prompt_weights", status, failed)) Py_RETURN_NONE;
+  if (failed) return nullptr;
   Py_RETURN_TRUE;
 }
 
@@ -197,10 +227,13 @@ PyObject* evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
       !flat(lo, at::kInt, dev, M) || lo->data_ptr() == lens || (wo && !flat(wo, at::kFloat, dev, M, kvh, cap)) ||
       (po && !flat(po, at::kInt, dev, M, kvh, cap)))
     Py_RETURN_NONE;
+  launched = true;
   const int status = f_evict(kv, M, ptr<const float>(w), wo ? ptr<float>(wo) : ptr<float>(w), ptr<const int>(p),
                              po ? ptr<int>(po) : ptr<int>(p), cap, ptr<const int>(next), (int)keep, (int)recent,
                              (int)sinks, ptr<int>(lo), ws, ws_bytes, stream);
-  if (status != ARIA_Q4_OK) Py_RETURN_NONE;
+  bool failed;
+  if (refused("aria_cache_evict", status, failed)) Py_RETURN_NONE;
+  if (failed) return nullptr;
   Py_RETURN_TRUE;
 }
 
@@ -278,9 +311,12 @@ PyObject* logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     made_token = at::empty({M}, x->options().dtype(at::kInt));
     token = &made_token;
   }
+  launched = true;
   const int status = f_logits(&r, x->data_ptr(), type, x_row, (int)M, (int)V, out->data_ptr(), out_type, y_row,
                               ptr<int>(token), ws, ws_bytes, stream);
-  if (status != ARIA_Q4_OK) Py_RETURN_NONE;
+  bool failed;
+  if (refused("aria_logits_adjust", status, failed)) Py_RETURN_NONE;
+  if (failed) return nullptr;
   PyObject* res = PyTuple_New(2);
   if (!res) return nullptr;
   if (made.defined()) {
@@ -298,21 +334,29 @@ PyObject* logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return res;
 }
 
-// no C++ exception leaves a C entry: the long way then meets the same trouble and says so
+// no C++ exception leaves a C entry: before a launch the long way meets the same trouble and
+// says so, after one it raises
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  launched = false;
   try {
     return F(self, args, n);
+  } catch (const std::exception& e) {
+    PyErr_Clear();
+    if (!launched) Py_RETURN_NONE;
+    PyErr_SetString(PyExc_RuntimeError, e.what());
   } catch (...) {
     PyErr_Clear();
-    Py_RETURN_NONE;
+    if (!launched) Py_RETURN_NONE;
+    PyErr_SetString(PyExc_RuntimeError, "unknown C++ exception");
   }
+  return nullptr;
 }
 
-// the four entry points' addresses
+// the four entry points' addresses, and what raises the meaning of a status
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 4) {
-    PyErr_SetString(PyExc_TypeError, "bind takes four addresses");
+  if (n != 5) {
+    PyErr_SetString(PyExc_TypeError, "bind takes four addresses and a function");
     return nullptr;
   }
   f_attention = reinterpret_cast<decltype(f_attention)>(PyLong_AsVoidPtr(args[0]));
@@ -320,6 +364,8 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   f_evict = reinterpret_cast<decltype(f_evict)>(PyLong_AsVoidPtr(args[2]));
   f_logits = reinterpret_cast<decltype(f_logits)>(PyLong_AsVoidPtr(args[3]));
   if (PyErr_Occurred()) return nullptr;
+  Py_XDECREF(check);
+  check = Py_NewRef(args[4]);
   Py_RETURN_NONE;
 }
 
