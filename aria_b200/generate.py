@@ -47,7 +47,8 @@ class BoundedDecoder(Decoder):
         self.weights = [torch.zeros(shape, dtype=torch.float32, device=device) for _ in self.kv]
         self.slot_pos = [torch.zeros(shape, dtype=torch.int32, device=device) for _ in self.kv]
         self._prompt_pos = torch.arange(cap, dtype=torch.int32, device=device).expand(shape)
-        self.used = 0  # slots in use, the same for every sequence
+        self.used = 0      # slots in use, the same for every sequence
+        self.position = 0  # of the next token, the same for every sequence
 
     def _attend(self, i: int) -> None:
         M, H, dh = self.M, self.cfg.num_heads, self.cfg.head_dim
@@ -65,38 +66,65 @@ class BoundedDecoder(Decoder):
         self.lens.copy_(self._lens_next)
         self.used = self.budget
 
-    def prefill(self, tokens, fill_cache: bool = True) -> torch.Tensor:
-        """The whole prompts [M][T]; afterwards the caches hold at most `budget` slots and
+    def run_prefill(self, T: int, fill_cache: bool = True, after_attention=None) -> torch.Tensor:
+        """Decoder.run_prefill; with fill_cache the caches then hold at most `budget` slots and
         self.positions the position of the next token."""
         if not fill_cache:
-            return super().prefill(tokens, False)
-        tok = torch.as_tensor(tokens, dtype=torch.int32)
-        if tok.dim() != 2 or tok.shape[0] != self.M:
-            raise ValueError(f"tokens must be [{self.M}][T]")
-        T, (M, H, dh) = tok.shape[1], (self.M, self.cfg.num_heads, self.cfg.head_dim)
+            return super().run_prefill(T, False, after_attention)
+        M, H, dh = self.M, self.cfg.num_heads, self.cfg.head_dim
 
         def count(i, qkv, lse):
             x = qkv.view(M, T, 3, H, dh)
             prompt_weights(x[:, :, 0], x[:, :, 1], lse, out=self.weights[i])
             self.slot_pos[i].copy_(self._prompt_pos)
+            if after_attention is not None:
+                after_attention(i, qkv, lse)
 
-        self._prefill_buffers(T)["tok"].copy_(tok.reshape(-1))
-        logits = self.run_prefill(T, True, after_attention=count)
+        logits = super().run_prefill(T, True, count)
         self.positions.fill_(T)
         self.lens.fill_(T)
-        self.used = T
+        self.used = self.position = T
         self._evict()
         return logits
 
-    def advance(self) -> torch.Tensor:
-        """One step for self.tokens at self.positions; returns the f32 logits [M][vocab]."""
-        logits = self.run()
+    def run(self) -> torch.Tensor:
+        """One step for self.tokens at self.positions, after which both the lengths and the
+        positions stand at the next token; returns the f32 logits [M][vocab].  (Decoder.run
+        leaves positions to the caller; here the caches' lengths move with them.)  Not for
+        graphs: when to evict is decided on the host."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a BoundedDecoder's step cannot be captured: evictions are decided on the host")
+        logits = super().run()
         self.positions.add_(1)
         self.lens.add_(1)
         self.used += 1
+        self.position += 1
         if self.used >= self.budget + self.slack:
             self._evict()
         return logits
+
+    def advance(self) -> torch.Tensor:
+        """run() under the name that says what it does."""
+        return self.run()
+
+    def step(self, tokens, positions=None) -> torch.Tensor:
+        """The next token of every sequence.  Tokens are stored in the order of the calls, so
+        positions, where given, have to be the next ones: self.position for every sequence."""
+        if positions is not None:
+            at = torch.as_tensor(positions).reshape(-1).tolist()
+            if at != [self.position] * self.M:
+                raise ValueError(f"the next position of every sequence is {self.position}, got {at}")
+        self.tokens.copy_(torch.as_tensor(tokens, dtype=torch.int32))
+        return self.run()
+
+    @property
+    def launches(self) -> int:
+        """Kernels of one run, without the evictions that come every `slack` steps."""
+        return super().launches + self.cfg.num_layers
+
+    def prefill_launches(self, fill_cache: bool = True) -> int:
+        """Kernels of one run_prefill, without the eviction at its end."""
+        return super().prefill_launches(fill_cache) + (self.cfg.num_layers if fill_cache else 0)
 
     def generate(self, prompts, steps: int, *, repetition: float = 1.0, frequency: float = 0.0, presence: float = 0.0,
                  bias_tokens: torch.Tensor | None = None, bias_values: torch.Tensor | None = None,
