@@ -125,6 +125,7 @@ class Decoder:
     def __init__(self, weights: DecoderWeights, M: int = 1, device="cuda"):
         cfg = weights.cfg
         self.w, self.cfg, self.M = weights, cfg, M
+        self.pos_embed = weights.pos_embed
         d, ff, V = cfg.d_model, cfg.ffn_dim, cfg.vocab_size
         self.k_cache = [torch.zeros(M, weights.max_seq, d, dtype=torch.float16, device=device)
                         for _ in range(cfg.num_layers)]
@@ -154,7 +155,7 @@ class Decoder:
         self.tokens / self.positions (device int32 [M]); returns self.logits."""
         cfg, w = self.cfg, self.w
         d = cfg.d_model
-        call("aria_embed_f16", w.embed.data_ptr(), w.pos_embed.data_ptr(), cfg.vocab_size, w.max_seq, d,
+        call("aria_embed_f16", w.embed.data_ptr(), self.pos_embed.data_ptr(), cfg.vocab_size, self.pos_embed.shape[0], d,
              self.tokens.data_ptr(), self.positions.data_ptr(), self.M, self.h.data_ptr(), _stream())
         fused_ln = self.M <= 64  # LayerNorm as the prologue of QKV / ffn_up (register-fed kernel)
         for i, p in enumerate(w.layers):

@@ -20,7 +20,7 @@ import argparse
 
 import torch
 
-from .decoder import Decoder, DecoderWeights
+from .decoder import Decoder, DecoderWeights, sinusoidal_positions
 from .logits import adjust
 from .paged import PagedKV, attention_paged, evict, prompt_weights
 
@@ -30,7 +30,8 @@ __all__ = ["BoundedDecoder"]
 class BoundedDecoder(Decoder):
     """A Decoder whose caches (weights.max_seq slots per sequence, in pages) never hold
     more than budget + slack slots of a sequence after its prompt.  recent, sinks: the
-    newest and first positions that are always kept."""
+    newest and first positions that are always kept.  Sequences grow past max_seq: their
+    position table, a formula, is extended as they do."""
 
     def __init__(self, weights: DecoderWeights, M: int = 1, *, budget: int = 256, recent: int = 32, sinks: int = 4,
                  slack: int = 16, page_size: int = 16, device="cuda"):
@@ -55,6 +56,14 @@ class BoundedDecoder(Decoder):
         x = self.qkv.view(M, 3, H, dh)
         attention_paged(x[:, 0], self.kv[i], k_new=x[:, 1], v_new=x[:, 2], out=self.att.view(M, H, dh),
                         weights=self.weights[i], slot_pos=self.slot_pos[i], positions=self.positions)
+
+    def _reach(self, positions: int) -> None:
+        """Rows of the position table for this many positions."""
+        rows = self.pos_embed.shape[0]
+        if positions > rows:
+            table = sinusoidal_positions(max(positions, 2 * rows), self.cfg.d_model, self.pos_embed.device)
+            table[:rows] = self.pos_embed
+            self.pos_embed = table
 
     def _evict(self) -> None:
         """Every layer's rows down to the budget (they share one length)."""
@@ -94,6 +103,7 @@ class BoundedDecoder(Decoder):
         graphs: when to evict is decided on the host."""
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a BoundedDecoder's step cannot be captured: evictions are decided on the host")
+        self._reach(self.position + 1)
         logits = super().run()
         self.positions.add_(1)
         self.lens.add_(1)
@@ -135,6 +145,7 @@ class BoundedDecoder(Decoder):
         prompts = torch.as_tensor(prompts, dtype=torch.int32)
         M, T = self.M, prompts.shape[1]
         dev = self.h.device
+        self._reach(T + steps)
         history = torch.zeros(M, T + steps, dtype=torch.int32, device=dev)
         logits = self.prefill(prompts).view(M, T, -1)[:, -1].float().contiguous()
         history[:, :T] = prompts.to(dev)

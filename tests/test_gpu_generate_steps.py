@@ -92,3 +92,24 @@ def test_a_capture_is_refused(weights):
     torch.cuda.synchronize()
     assert b.used == b.position == 10
     b.step([3])
+
+
+def test_positions_past_the_cache_have_their_own_embedding(weights):
+    """Bounded caches of 128 slots, sequences of 230 positions: the logits are those of weights whose
+    position table was made for 512, bit for bit (nothing else depends on max_seq)."""
+    from aria_b200.decoder import DecoderWeights
+    from aria_b200.generate import BoundedDecoder
+    M, T, steps = 2, 90, 140
+    wide = DecoderWeights(weights.cfg, max_seq=512)
+    kw = dict(budget=48, recent=8, sinks=2, slack=8)
+    a, b = BoundedDecoder(weights, M, **kw), BoundedDecoder(wide, M, **kw)
+    p = _prompts(M, T)
+    assert torch.equal(a.prefill(p), b.prefill(p))
+    for s in range(steps):
+        tok = torch.full((M,), (37 * s) % 1000, dtype=torch.int32, device="cuda")
+        for d in (a, b):
+            d.tokens.copy_(tok)
+        assert torch.equal(a.advance(), b.advance()), T + s
+    assert a.positions.tolist() == [T + steps] * M
+    assert torch.equal(BoundedDecoder(weights, M, **kw).generate(p, steps),
+                       BoundedDecoder(wide, M, **kw).generate(p, steps))
