@@ -120,14 +120,18 @@ def _stream() -> int:
 
 class Decoder:
     """M sequences decoding together, one token each per `step`, with their
-    KV caches ([layer] f16 [M][max_seq][d], K and V) on the device."""
+    KV caches ([layer] f16 [M][max_seq][d], K and V) on the device.  cache_rows: the
+    caches' rows per sequence where they are to be more than max_seq."""
 
-    def __init__(self, weights: DecoderWeights, M: int = 1, device="cuda"):
+    def __init__(self, weights: DecoderWeights, M: int = 1, device="cuda", cache_rows: int | None = None):
         cfg = weights.cfg
         self.w, self.cfg, self.M = weights, cfg, M
         self.pos_embed = weights.pos_embed
         d, ff, V = cfg.d_model, cfg.ffn_dim, cfg.vocab_size
-        self.k_cache = [torch.zeros(M, weights.max_seq, d, dtype=torch.float16, device=device)
+        rows = weights.max_seq if cache_rows is None else cache_rows
+        if rows < weights.max_seq:
+            raise ValueError(f"the caches need at least max_seq = {weights.max_seq} rows")
+        self.k_cache = [torch.zeros(M, rows, d, dtype=torch.float16, device=device)
                         for _ in range(cfg.num_layers)]
         self.v_cache = [torch.zeros_like(k) for k in self.k_cache]
         self.h = torch.empty(M, d, dtype=torch.float32, device=device)
@@ -147,7 +151,7 @@ class Decoder:
         """Layer i's attention of the new tokens: self.qkv -> self.att, their keys and
         values into the caches."""
         call("aria_attention_decode", self.qkv.data_ptr(), self.M, self.cfg.d_model, self.cfg.num_heads,
-             self.k_cache[i].data_ptr(), self.v_cache[i].data_ptr(), self.w.max_seq, self.positions.data_ptr(),
+             self.k_cache[i].data_ptr(), self.v_cache[i].data_ptr(), self.k_cache[i].shape[1], self.positions.data_ptr(),
              self.att.data_ptr(), _stream())
 
     def run(self) -> torch.Tensor:

@@ -35,10 +35,12 @@ class BoundedDecoder(Decoder):
 
     def __init__(self, weights: DecoderWeights, M: int = 1, *, budget: int = 256, recent: int = 32, sinks: int = 4,
                  slack: int = 16, page_size: int = 16, device="cuda"):
-        super().__init__(weights, M, device)
-        cfg, cap = self.cfg, weights.max_seq
-        if not 0 < budget <= budget + slack < cap or recent + sinks > budget:
-            raise ValueError(f"needs recent + sinks <= budget and budget + slack < max_seq = {cap}")
+        if page_size <= 0 or not 0 < budget <= budget + slack < weights.max_seq or recent + sinks > budget:
+            raise ValueError("needs a page_size, recent + sinks <= budget and budget + slack < max_seq = "
+                             f"{weights.max_seq}")
+        cap = -(-weights.max_seq // page_size) * page_size  # whole pages
+        super().__init__(weights, M, device, cache_rows=cap)
+        cfg = self.cfg
         self.budget, self.recent, self.sinks, self.slack = budget, recent, sinks, slack
         self.lens = torch.zeros(M, dtype=torch.int32, device=device)
         self._lens_next = torch.zeros_like(self.lens)

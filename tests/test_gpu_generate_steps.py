@@ -113,3 +113,26 @@ def test_positions_past_the_cache_have_their_own_embedding(weights):
     assert a.positions.tolist() == [T + steps] * M
     assert torch.equal(BoundedDecoder(weights, M, **kw).generate(p, steps),
                        BoundedDecoder(wide, M, **kw).generate(p, steps))
+
+
+def test_lengths_that_are_no_multiple_of_a_page():
+    """max_seq 101 in pages of 16 and of 7: the same tokens as in pages of 1 (whose slots are the same)."""
+    from aria_b200.decoder import DecoderWeights
+    from aria_b200.efkolos import EfkolosConfig
+    from aria_b200.generate import BoundedDecoder
+    w = DecoderWeights(EfkolosConfig(num_layers=1, d_model=128, num_heads=2, ffn_dim=256, vocab_size=200), max_seq=101)
+    p = torch.randint(0, 200, (2, 101), generator=torch.Generator().manual_seed(1))
+    tokens = [BoundedDecoder(w, 2, budget=80, slack=20, page_size=ps).generate(p, 40) for ps in (1, 16, 7)]
+    assert torch.equal(tokens[0], tokens[1]) and torch.equal(tokens[0], tokens[2])
+
+
+@pytest.mark.parametrize("prompt", [40, 41, 401])
+def test_the_command(monkeypatch, capsys, prompt):
+    """python -m aria_b200.generate for prompts of any length."""
+    import sys
+
+    from aria_b200 import generate
+    monkeypatch.setattr(sys, "argv", ["generate", "--prompt", str(prompt), "--tokens", "9", "--budget", "48", "--layers",
+                                      "1"])
+    generate.main()
+    assert f"2 sequences x ({prompt} + 9) tokens" in capsys.readouterr().out
