@@ -29,7 +29,9 @@
 //               block, a quarter of the queries each: 55 us at 4 x 2048 x 14 heads;
 //               two warps: 70 us, the unit 40% busy; so: 41 us.)
 //   warp 18     lse rows of the query blocks -> shared memory, negated, in the log2 domain;
-//               -inf for queries before `first` or past the end, whose terms vanish
+//               -inf for queries before `first` or past the end, whose terms vanish, and
+//               for those whose lse is -inf, with a word by which the block's scores are
+//               looked at first (theirs need not be finite)
 //   warp 19     adds an item's four sums per key and stores them
 // Every wait is bounded (one second for the MMA issuer, two for the others; an abort
 // flag; the code in this unit's g_device_error).
@@ -159,6 +161,27 @@ __device__ __forceinline__ void exp2_poly2(float& x, float& y) {
   y = y >= -126.0f ? __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23)) : y0;
 }
 
+// The terms of one block of queries, each taken by selection: those from cmin on that saw
+// something.  neg_lse: the block's.  (Beside the unrolled loop, not in it: a test there for
+// blocks that hardly occur took 46 us to 51 at 4 x 2048 x 14 heads.)
+__device__ __forceinline__ uint64_t prompt_selected(uint32_t s_col, const float* neg_lse, int cmin, float scale_log2) {
+  float sum = 0.0f;
+#pragma unroll 1
+  for (int c = 0; c < kPwB; c += 16) {
+    uint32_t sv[16];
+    tc::tmem_ld_32x32b_x16(s_col + c, sv);
+    tc::tmem_ld_wait();
+    tc::reg_tie(sv);
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      const float l = neg_lse[c + e];
+      const float p = tc::ex2_approx(fmaf(__uint_as_float(sv[e]), scale_log2, l));
+      sum += c + e >= cmin && l != -INFINITY ? p : 0.0f;
+    }
+  }
+  return pack2(__float_as_uint(sum), 0u);
+}
+
 template <int DH, bool BF16>
 __global__ void __launch_bounds__(kPwThreads, 1)
     prompt_weights_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -178,6 +201,7 @@ __global__ void __launch_bounds__(kPwThreads, 1)
   uint64_t* mma_drain = p_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_drain + 1);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  int* lse_gaps = abort_flag + 1;  // [kPwS] whether some query of the block saw nothing
   float* lse_s = reinterpret_cast<float*>(smem + L::kLseOff);
   float* part_sum = reinterpret_cast<float*>(smem + L::kSumOff);
   auto give_up = [&](int wait_result, int code) {
@@ -339,10 +363,22 @@ __global__ void __launch_bounds__(kPwThreads, 1)
       for (; j < blocks; j += kPwS, uses++) {
         if (!wait(&s_full[b], uses & 1, tc::kErrTimeoutFull)) break;
         tc::tc_fence_after();
-        const int q0 = (im.q0 + qb) * kPwB;
-        for (qb += kPwS; qb >= im.nq;) qb -= im.nq;
         uint32_t sv[2][16];
         tc::tmem_ld_32x32b_x16(s_col, sv[0]);
+        const int q0 = (im.q0 + qb) * kPwB;
+        for (qb += kPwS; qb >= im.nq;) qb -= im.nq;
+        if (lse_gaps[b] != 0) {  // queries that saw nothing: their scores need not be finite
+          tc::tmem_ld_wait();
+          tc::reg_tie(sv[0]);
+          sum[0] = add2(sum[0], prompt_selected(s_col, lse_s + b * kPwB, max(key, a.first) - q0, a.scale_log2));
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            tc::mbar_arrive(&s_empty[b]);
+            tc::mbar_arrive(&l_empty[b]);
+          }
+          continue;
+        }
 #pragma unroll
         for (int c = 0; c < 8; c++) {
           tc::tmem_ld_wait();
@@ -457,38 +493,66 @@ __global__ void __launch_bounds__(kPwThreads, 1)
     }
   } else if (warp == 2 + kPwSumWarps) {
     // ------------------------------------------------------------ lse rows
-    int g = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; t < n_items && ok; t += gridDim.x) {
-      const PromptItem im = prompt_item(a, t, n_items);
-      int h = im.nq > 0 ? im.lo / im.nq : 0, qb = im.lo - h * im.nq;
-      for (int j = im.lo; j < im.hi; j++, g++) {
-        const float* row = a.lse + ((size_t)im.seq * a.Hkv * a.G + im.hk * a.G + h) * a.T;
-        const int b = g % kPwS;
-        float v[4];
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-          const int q = (im.q0 + qb) * kPwB + 32 * u + lane;
-          v[u] = q < a.T && q >= a.first ? row[q] * -1.4426950408889634f : -INFINITY;
-          if (v[u] == INFINITY) v[u] = -INFINITY;  // a row that saw nothing gives nothing
-        }
-        if (g >= kPwS) {
-          const int w = tc::mbar_wait_or_abort(&l_empty[b], ((g / kPwS) - 1) & 1, 2 * a.wait_ns, abort_flag);
-          if (!__all_sync(0xffffffffu, w == tc::kWaitOk)) {
-            if (lane == 0) give_up(w, tc::kErrTimeoutEmpty);
-            ok = false;
-            break;
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 4; u++) lse_s[b * kPwB + 32 * u + lane] = v[u];
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&s_full[b]);
-        if (++qb == im.nq) {
-          qb = 0;
-          h++;
+    // (a block's rows are fetched while the one before it waits for its buffer)
+    int t = blockIdx.x, j = 0, h = 0, qb = 0;
+    PromptItem im;
+    auto begin = [&]() {  // the first block of item t, or of the first one after it that has any
+      for (; t < n_items; t += gridDim.x) {
+        im = prompt_item(a, t, n_items);
+        if (im.lo < im.hi) {
+          j = im.lo;
+          h = im.lo / im.nq;
+          qb = im.lo - h * im.nq;
+          return;
         }
       }
+    };
+    float next[4];
+    auto fetch = [&]() {
+      if (t >= n_items) return;
+      const float* row = a.lse + ((size_t)im.seq * a.Hkv * a.G + im.hk * a.G + h) * a.T;
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int q = (im.q0 + qb) * kPwB + 32 * u + lane;
+        next[u] = q < a.T && q >= a.first ? row[q] : INFINITY;
+      }
+      if (++qb == im.nq) {
+        qb = 0;
+        h++;
+      }
+      if (++j == im.hi) {
+        t += gridDim.x;
+        begin();
+      }
+    };
+    begin();
+    bool more = t < n_items;
+    fetch();
+    for (int g = 0; more; g++) {
+      const int b = g % kPwS;
+      float v[4];
+      bool gap = false;
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        v[u] = next[u] * -1.4426950408889634f;
+        gap |= v[u] == INFINITY;  // a row that saw nothing gives nothing
+        if (v[u] == INFINITY) v[u] = -INFINITY;
+      }
+      gap = __any_sync(0xffffffffu, gap);
+      more = t < n_items;
+      fetch();
+      if (g >= kPwS) {
+        const int w = tc::mbar_wait_or_abort(&l_empty[b], ((g / kPwS) - 1) & 1, 2 * a.wait_ns, abort_flag);
+        if (!__all_sync(0xffffffffu, w == tc::kWaitOk)) {
+          if (lane == 0) give_up(w, tc::kErrTimeoutEmpty);
+          break;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; u++) lse_s[b * kPwB + 32 * u + lane] = v[u];
+      if (lane == 0) lse_gaps[b] = gap;
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&s_full[b]);
     }
   }
 

@@ -29,3 +29,19 @@ def test_a_nan_query_makes_the_weights_of_its_keys_nan(residue, dh):
     got = _f64(prompt_weights(q, k, torch.from_numpy(rows)[None].float().cuda())[0, 0])
     assert np.isnan(got[:t + 1]).all()
     assert np.all(np.abs(got[t + 1:] - ref[0, t + 1:]) <= 5e-5 * ref[0, t + 1:] + 1e-6)
+
+
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("value", ["nan", "inf", "-inf"])
+def test_rows_that_saw_nothing_give_nothing_whatever_they_hold(value, dh):
+    """Queries with lse -inf whose rows hold NaN or infinities, in several blocks, among sound ones."""
+    from aria_b200.paged import prompt_weights
+    g = torch.Generator(device="cuda").manual_seed(dh)
+    T, hidden = 700, [0, 1, 130, 131, 255, 400, 402, 403, 699]
+    q, k = (torch.randn(1, T, 2, dh, generator=g, device="cuda").half() for _ in range(2))
+    _, rows = paged_np.prompt_weights(_f64(q[0]), _f64(k[0]), dh ** -0.5)
+    rows[1, hidden] = -np.inf
+    ref, _ = paged_np.prompt_weights(_f64(q[0]), _f64(k[0]), dh ** -0.5, 0, rows)
+    q[0, hidden, 1, 11] = float(value)
+    got = _f64(prompt_weights(q, k, torch.from_numpy(rows)[None].float().cuda())[0])
+    assert np.all(np.abs(got - ref) <= 5e-5 * ref + 1e-6)
