@@ -82,6 +82,13 @@ def _want(t: torch.Tensor, name: str, dtype, shape, dev: int) -> int:
     return t.data_ptr()
 
 
+def _int32(**values) -> None:
+    """The C ABI's counts are 32-bit; ctypes would cut larger ones off in silence."""
+    for name, v in values.items():
+        if not -2**31 <= v < 2**31:
+            raise ValueError(f"{name} = {v} does not fit 32 bits")
+
+
 class PagedKV:
     """One layer's cache.  k_pages, v_pages: f16 or bf16 [num_pages][page_size]
     [kv_heads][head_dim], any strides that are multiples of 8 with contiguous head
@@ -248,6 +255,7 @@ def prompt_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, out: 
         if fastcall().prompt(q, k, lse, out, scale if scale is not None else 1.0 / math.sqrt(q.shape[-1]), first_query,
                              ws[0], ws[1], stream):
             return out
+    _int32(first_query=first_query)
     if q.dim() != 4 or k.dim() != 4 or q.dtype not in _DTYPES or k.dtype is not q.dtype or not q.is_cuda:
         raise TypeError("q and k must be 4-D f16 or bf16 CUDA tensors of one type")
     B, T, heads, dh = q.shape
@@ -296,6 +304,7 @@ def evict(kv: PagedKV, weights: torch.Tensor, slot_pos: torch.Tensor, next_pos: 
     if fastcall().evict(kv._ref, kv.M, kv.kv_heads, dev, kv._lens_ptr, keep, recent, sinks, ws[0], ws[1], stream, weights,
                         slot_pos, next_pos, weights_out, slot_pos_out, lens_out):
         return lens_out
+    _int32(keep=keep, recent=recent, sinks=sinks)
     shape = weights.shape
     if weights.dim() != 3 or shape[:2] != (kv.M, kv.kv_heads):
         raise ValueError("weights must be [M][kv_heads][cap]")

@@ -72,3 +72,23 @@ def test_a_refusal_goes_the_long_way(answered, name):
     calls = answered(OK)
     run()
     assert calls == ["fast"]
+
+
+@pytest.mark.parametrize("n", [2**31, 2**32 + 5, -2**31 - 1, 2**40 + 20])
+def test_counts_past_32_bits_are_refused(n):
+    """Refused, not cut to what the lower 32 bits say."""
+    from aria_b200.paged import PagedKV, evict, prompt_weights
+    k, v = (torch.zeros(4, 16, 2, 64, device="cuda").half() for _ in range(2))
+    kv = PagedKV(k, v, torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4),
+                 torch.tensor([50], dtype=torch.int32, device="cuda"))
+    w, p = torch.rand(1, 2, 64, device="cuda"), torch.arange(64, dtype=torch.int32, device="cuda").expand(
+        1, 2, 64).contiguous()
+    w0 = w.clone()
+    for kw in (dict(keep=n), dict(keep=40, recent=n), dict(keep=40, sinks=n)):
+        with pytest.raises(ValueError):
+            evict(kv, w, p, kv.lens + 1, **kw)
+    assert torch.equal(w, w0)
+    x, lse = torch.zeros(1, 8, 2, 64, device="cuda").half(), torch.zeros(1, 2, 8, device="cuda")
+    for out in (None, torch.zeros(1, 2, 8, device="cuda")):
+        with pytest.raises(ValueError):
+            prompt_weights(x, x, lse, out=out, first_query=n)
