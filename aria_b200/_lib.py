@@ -8,7 +8,9 @@ kernels behind the C ABI.
 from __future__ import annotations
 
 import ctypes
+import importlib.metadata
 import os
+import sys
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libaria_q4.so")
@@ -125,13 +127,34 @@ def _lib() -> ctypes.CDLL:
 _FAST = None
 
 
+def fastcall_key() -> str | None:
+    """The Python and the torch that a build of aria_b200._fastcall is for, None without torch."""
+    try:
+        return f"{sys.implementation.cache_tag} torch {importlib.metadata.version('torch')}"
+    except importlib.metadata.PackageNotFoundError:
+        return None
+
+
+class _LongWay:
+    """In place of aria_b200._fastcall where it was not built, or not for this torch: every
+    call goes the long way, through ctypes."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
 def fastcall():
-    """The C++ binding of the serving operators (aria_b200/_fastcall.so), bound to the
-    library's entry points; like the library it has to have been built."""
+    """The C++ binding of the serving operators, bound to the library's entry points."""
     global _FAST
     if _FAST is None:
         import torch  # noqa: F401  (loads what the module links against)
-        from . import _fastcall
+        try:
+            from . import _fastcall
+        except ImportError:
+            _fastcall = None
+        if _fastcall is None or _fastcall.key != fastcall_key():
+            _FAST = _LongWay()
+            return _FAST
         lib = _lib()
         _fastcall.bind(*(ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in (
             "aria_attention_paged", "aria_prompt_weights", "aria_cache_evict", "aria_logits_adjust")), check)

@@ -5,8 +5,10 @@
 
 The library is a plain C-ABI shared object (include/aria_q4.h) with the CUDA
 runtime linked statically, so any host language can dlopen it; Python reaches it
-through ctypes (aria_b200/_lib.py).  Objects go to aria_b200/_build/.  The serving operators
-have a second, shorter way from Python, aria_b200/_fastcall.so (csrc/fastcall.cpp).
+through ctypes (aria_b200/_lib.py).  Objects go to aria_b200/_build/.  nvcc and its host
+compiler are all that it needs.  Where torch is installed with its headers, the serving
+operators get a second, shorter way from Python, the module aria_b200._fastcall
+(csrc/fastcall.cpp), built for this Python and this torch.
 """
 from __future__ import annotations
 
@@ -15,13 +17,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libaria_q4.so")
-FASTCALL = os.path.join(PKG, "_fastcall.so")
+FASTCALL = os.path.join(PKG, "_fastcall" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 SOURCES = ["q4_pack.cu", "q4_gemv.cu", "q4_decode.cu", "q4_gemm_tc.cu", "q4_layer.cu", "attn_prefill.cu",
            "attn_paged.cu", "prompt_weights.cu", "cache_evict.cu", "logits.cu", "p2p_allreduce.cu", "q4_capi.cu",
            "paged_capi.cu"]
@@ -48,25 +51,35 @@ def _newer(target: str, deps: list[str]) -> bool:
     return any(os.path.exists(d) and os.path.getmtime(d) > t for d in deps)
 
 
-def build_fastcall(force: bool = False) -> str:
-    """aria_b200/_fastcall.so: the C++ binding of the serving operators (host code only;
-    torch's headers and the libraries that `import torch` loads)."""
-    src = os.path.join(CSRC, "fastcall.cpp")
-    if force or _newer(FASTCALL, [src, os.path.join(ROOT, "include", "aria_q4.h")]):
-        import sysconfig
+def build_fastcall(force: bool = False) -> str | None:
+    """The C++ binding of the serving operators (host code only; torch's headers and the
+    libraries that `import torch` loads), or None where torch or its headers are absent."""
+    from ._lib import fastcall_key
+    key, src = fastcall_key(), os.path.join(CSRC, "fastcall.cpp")
+    key_file = os.path.join(OBJ, "fastcall.key")
+    if key is None:
+        return None
+    built = open(key_file).read() if os.path.exists(key_file) else ""
+    if not force and built == key and not _newer(FASTCALL, [src, os.path.join(ROOT, "include", "aria_q4.h")]):
+        return FASTCALL
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
 
-        import torch
-        from torch.utils.cpp_extension import include_paths, library_paths
-        # torch's headers name CUDA types even where no CUDA call is made
-        inc = [*include_paths(), sysconfig.get_paths()["include"],
-               os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
-        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *[f"-I{d}" for d in inc], src,
-               "-o", FASTCALL, *[f"-L{d}" for d in library_paths()], "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10"]
-        env = {k: v for k, v in os.environ.items() if k not in ("CC", "CXX")}
-        r = subprocess.run(cmd, capture_output=True, text=True, env=env)
-        if r.returncode != 0:
-            raise RuntimeError(f"g++ failed on fastcall.cpp:\n{r.stdout}\n{r.stderr}")
+    # torch's headers name CUDA types even where no CUDA call is made
+    inc = [*include_paths(), sysconfig.get_paths()["include"],
+           os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
+    if not any(os.path.exists(os.path.join(d, "ATen", "ATen.h")) for d in inc) or not any(
+            os.path.exists(os.path.join(d, "Python.h")) for d in inc):
+        return None
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f'-DFASTCALL_KEY="{key}"',
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *[f"-I{d}" for d in inc], src,
+           "-o", FASTCALL, *[f"-L{d}" for d in library_paths()], "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10"]
+    env = {k: v for k, v in os.environ.items() if k not in ("CC", "CXX")}
+    r = subprocess.run(cmd, capture_output=True, text=True, env=env)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on fastcall.cpp:\n{r.stdout}\n{r.stderr}")
+    with open(key_file, "w") as f:
+        f.write(key)
     return FASTCALL
 
 
@@ -98,7 +111,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True, env=env)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
-    build_fastcall(force)
+    if build_fastcall(force) is None:
+        sys.stderr.write("aria_b200: no torch headers here: without aria_b200._fastcall the serving operators' calls "
+                         "take a few microseconds longer\n")
     return LIB
 
 

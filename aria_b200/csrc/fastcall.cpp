@@ -380,4 +380,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fastcall", nullptr, -1, methods, 
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__fastcall(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__fastcall(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "key", FASTCALL_KEY) < 0) {  // the Python and the torch that it is for
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}
