@@ -68,12 +68,13 @@ def build_fastcall(force: bool = False) -> str | None:
     # torch's headers name CUDA types even where no CUDA call is made
     inc = [*include_paths(), sysconfig.get_paths()["include"],
            os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
-    if not any(os.path.exists(os.path.join(d, "ATen", "ATen.h")) for d in inc) or not any(
+    if torch.version.cuda is None or not any(os.path.exists(os.path.join(d, "ATen", "ATen.h")) for d in inc) or not any(
             os.path.exists(os.path.join(d, "Python.h")) for d in inc):
         return None
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f'-DFASTCALL_KEY="{key}"',
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *[f"-I{d}" for d in inc], src,
-           "-o", FASTCALL, *[f"-L{d}" for d in library_paths()], "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10"]
+           "-o", FASTCALL, *[f"-L{d}" for d in library_paths()], "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10",
+           "-lc10_cuda"]
     env = {k: v for k, v in os.environ.items() if k not in ("CC", "CXX")}
     r = subprocess.run(cmd, capture_output=True, text=True, env=env)
     if r.returncode != 0:

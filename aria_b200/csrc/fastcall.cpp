@@ -10,11 +10,13 @@
 // that does not pass, a workspace that has to grow, a call that the library refuses -- and
 // the Python code then goes the long way, which says what is wrong.  A CUDA error raises
 // here: one of a call's kernels may have run, and sums, moves and stored rows are not to
-// be made twice.  No arithmetic and no CUDA call happens here.
+// be made twice.  No arithmetic happens here, and of CUDA only the current device is asked:
+// a launch goes there, so tensors of another one take the long way, which changes it.
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAFunctions.h>
 
 #include <exception>
 
@@ -46,6 +48,8 @@ bool refused(const char* name, int status, bool& failed) {
   if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, name);
   return false;
 }
+
+bool elsewhere(int dev) { return c10::cuda::current_device() != dev; }
 
 struct Args {
   PyObject* const* a;
@@ -117,7 +121,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor *q = a.tensor(bad), *kn = a.tensor(bad), *vn = a.tensor(bad), *out = a.tensor(bad),
                    *w = a.tensor(bad), *wo = a.tensor(bad), *sp = a.tensor(bad), *pos = a.tensor(bad);
   if (PyErr_Occurred()) return nullptr;
-  if (bad || !q || q->dim() != 3 || !kn != !vn) Py_RETURN_NONE;
+  if (bad || !q || q->dim() != 3 || !kn != !vn || elsewhere(dev)) Py_RETURN_NONE;
   const at::ScalarType type = kv->dtype == ARIA_Q4_BF16 ? at::kBFloat16 : at::kHalf;
   const int64_t heads = q->size(1);
   long long qr, qh, nr = 0, nh = 0, vr = 0, vh = 0, orow, oh;
@@ -182,6 +186,7 @@ PyObject* prompt(PyObject*, PyObject* const* args, Py_ssize_t n) {
       first < 0 || first > 0x7fffffff)
     Py_RETURN_NONE;
   const int dev = q->get_device();
+  if (elsewhere(dev)) Py_RETURN_NONE;
   const at::ScalarType type = q->scalar_type();
   const int64_t B = q->size(0), T = q->size(1), heads = q->size(2), dh = q->size(3), kvh = k->size(2);
   if ((type != at::kHalf && type != at::kBFloat16) || !on(*k, type, dev) || k->size(0) != B || k->size(1) != T ||
@@ -220,7 +225,7 @@ PyObject* evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (PyErr_Occurred()) return nullptr;
   const long long most = 0x7fffffff;
   if (bad || !w || !p || !next || !lo || w->dim() != 3 || keep > most || recent > most || sinks > most || keep <= 0 ||
-      recent < 0 || sinks < 0)
+      recent < 0 || sinks < 0 || elsewhere(dev))
     Py_RETURN_NONE;
   const int64_t cap = w->size(2);
   if (!flat(w, at::kFloat, dev, M, kvh, cap) || !flat(p, at::kInt, dev, M, kvh, cap) || !flat(next, at::kInt, dev, M) ||
@@ -255,7 +260,7 @@ PyObject* logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (bad || !x || !x->is_cuda() || x->dim() != 2) Py_RETURN_NONE;
   const int dev = x->get_device(), type = type_code(x->scalar_type());
   const int64_t M = x->size(0), V = x->size(1);
-  if (type < 0 || M == 0 || M > 65535 || V <= 0 || V > 0x7fffffff) Py_RETURN_NONE;
+  if (elsewhere(dev) || type < 0 || M == 0 || M > 65535 || V <= 0 || V > 0x7fffffff) Py_RETURN_NONE;
   const long long x_row = matrix(*x, x->scalar_type(), dev, M);
   if (x_row < 0) Py_RETURN_NONE;
   aria_logit_rules r = {};

@@ -64,18 +64,18 @@ def adjust(logits: torch.Tensor, *, out: torch.Tensor | None = None, history: to
     result, -1 where nothing is left above -inf."""
     dev = logits.get_device()  # -1 on the CPU
     if dev >= 0:
-        if _current_device() != dev:  # a launch goes to the current device
-            with torch.cuda.device(dev):
-                return adjust(logits, out=out, history=history, history_lens=history_lens, prompt_lens=prompt_lens,
-                              repetition=repetition, frequency=frequency, presence=presence, bias_tokens=bias_tokens,
-                              bias_values=bias_values, allowed=allowed, want_token=want_token, token=token)
         stream = _stream(dev)
         ws = _held("logits", dev, stream)
         r = fastcall().logits(ws[0], ws[1], stream, want_token, logits, out, history, history_lens, prompt_lens,
                               repetition, frequency, presence, bias_tokens, bias_values, allowed, token)
         if r is not None:
             return r
-    # the first call on a stream, one that needs more scratch, or something to say
+        if _current_device() != dev:  # a launch goes to the current device
+            with torch.cuda.device(dev):
+                return adjust(logits, out=out, history=history, history_lens=history_lens, prompt_lens=prompt_lens,
+                              repetition=repetition, frequency=frequency, presence=presence, bias_tokens=bias_tokens,
+                              bias_values=bias_values, allowed=allowed, want_token=want_token, token=token)
+    # another device is current, the first call on a stream, one that needs more scratch, or something to say
     if dev < 0 or logits.dim() != 2 or logits.dtype not in _DTYPES:
         raise TypeError("logits must be an f32, f16 or bf16 [M][V] CUDA tensor")
     M, V = logits.shape

@@ -184,18 +184,19 @@ def attention_paged(q: torch.Tensor, kv: PagedKV, *, k_new: torch.Tensor | None 
     weights f32 [M][kv_heads][cap >= kv.slots]: the running sums of the attention
     weight, updated in place or into weights_out; the new token's slot starts from 0,
     and its entry of slot_pos (int32, the same shape) becomes positions[m]."""
-    if _current_device() != kv.index:  # a launch goes to the current device
-        with torch.cuda.device(kv.index):
-            return attention_paged(q, kv, k_new=k_new, v_new=v_new, scale=scale, out=out, want_lse=want_lse,
-                                   weights=weights, weights_out=weights_out, slot_pos=slot_pos, positions=positions)
     stream = _stream(kv.index)
-    ws = _held("attn", kv.index, stream)
+    ws = _WORKSPACES.get(("attn", kv.index, 0), _NO_WORKSPACE) if stream == 0 else _held("attn", kv.index, stream)
     r = fastcall().attention(kv._ref, kv.M, kv.kv_heads, kv.head_dim, kv.index, kv._scale if scale is None else scale,
                              ws[0], ws[1], stream, want_lse, q, k_new, v_new, out, weights, weights_out, slot_pos,
                              positions)
     if r is not None:
         return r
-    # the first call on a stream, one that needs more scratch, or something to say
+    # another device is current, the first call on a stream, one that needs more scratch, or
+    # something to say
+    if _current_device() != kv.index:  # a launch goes to the current device
+        with torch.cuda.device(kv.index):
+            return attention_paged(q, kv, k_new=k_new, v_new=v_new, scale=scale, out=out, want_lse=want_lse,
+                                   weights=weights, weights_out=weights_out, slot_pos=slot_pos, positions=positions)
     shape = q.shape
     if len(shape) != 3 or shape[0] != kv.M or shape[2] != kv.head_dim or shape[1] == 0 or shape[1] % kv.kv_heads:
         raise ValueError(f"q must be [{kv.M}][heads][{kv.head_dim}] with heads a multiple of {kv.kv_heads}")
@@ -246,15 +247,15 @@ def prompt_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, out: 
     [B][kv_heads][>= T] tensor with contiguous rows (a new [B][kv_heads][T] one by
     default) and returns it.  head_dim 64 or 128."""
     dev = q.get_device()  # -1 on the CPU
-    if dev >= 0 and _current_device() != dev:
-        with torch.cuda.device(dev):
-            return prompt_weights(q, k, lse, out=out, scale=scale, first_query=first_query)
     if out is not None and dev >= 0:
         stream = _stream(dev)
         ws = _held("prompt", dev, stream)
         if fastcall().prompt(q, k, lse, out, scale if scale is not None else 1.0 / math.sqrt(q.shape[-1]), first_query,
                              ws[0], ws[1], stream):
             return out
+    if dev >= 0 and _current_device() != dev:
+        with torch.cuda.device(dev):
+            return prompt_weights(q, k, lse, out=out, scale=scale, first_query=first_query)
     _int32(first_query=first_query)
     if q.dim() != 4 or k.dim() != 4 or q.dtype not in _DTYPES or k.dtype is not q.dtype or not q.is_cuda:
         raise TypeError("q and k must be 4-D f16 or bf16 CUDA tensors of one type")
@@ -292,10 +293,6 @@ def evict(kv: PagedKV, weights: torch.Tensor, slot_pos: torch.Tensor, next_pos: 
     slots end with weight 0 and position -1.  Returns lens_out (int32 [M], another tensor
     than kv.lens) = min(lens, keep); copy it to kv.lens once every layer that shares kv.lens
     has been evicted from."""
-    if _current_device() != kv.index:
-        with torch.cuda.device(kv.index):
-            return evict(kv, weights, slot_pos, next_pos, keep, recent=recent, sinks=sinks, weights_out=weights_out,
-                         slot_pos_out=slot_pos_out, lens_out=lens_out)
     if lens_out is None:
         lens_out = torch.empty_like(kv.lens)
     dev = kv.index
@@ -304,6 +301,10 @@ def evict(kv: PagedKV, weights: torch.Tensor, slot_pos: torch.Tensor, next_pos: 
     if fastcall().evict(kv._ref, kv.M, kv.kv_heads, dev, kv._lens_ptr, keep, recent, sinks, ws[0], ws[1], stream, weights,
                         slot_pos, next_pos, weights_out, slot_pos_out, lens_out):
         return lens_out
+    if _current_device() != kv.index:
+        with torch.cuda.device(kv.index):
+            return evict(kv, weights, slot_pos, next_pos, keep, recent=recent, sinks=sinks, weights_out=weights_out,
+                         slot_pos_out=slot_pos_out, lens_out=lens_out)
     _int32(keep=keep, recent=recent, sinks=sinks)
     shape = weights.shape
     if weights.dim() != 3 or shape[:2] != (kv.M, kv.kv_heads):

@@ -78,6 +78,8 @@ def test_calls_are_made_with_the_tensors_device_current(monkeypatch):
     class Fast:
         def __getattr__(self, name):
             def record(*args):
+                if state["device"] != 1:  # as the binding itself: tensors of another device take the long way
+                    return None
                 state["calls"].append((name, state["device"], args))
                 return "made"
             return record
