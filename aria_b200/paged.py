@@ -67,7 +67,10 @@ def _workspace(kind: str, nbytes: int, dev: int, stream: int, cleared: str = "co
         t = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=torch.device("cuda", dev))
         t[:_lib.lib().aria_paged_workspace_counter_bytes() if cleared == "counters" else None].zero_()
         if _capturing():
-            ws = _GRAPH_WORKSPACES[kind, dev, stream] = (t.data_ptr(), t.numel(), t, _capture_id(stream))
+            graph = _capture_id(stream)
+            for key in [k for k, w in _GRAPH_WORKSPACES.items() if w[3] != graph]:
+                del _GRAPH_WORKSPACES[key]  # of captures before this one: their graphs' pools hold the memory
+            ws = _GRAPH_WORKSPACES[kind, dev, stream] = (t.data_ptr(), t.numel(), t, graph)
         else:
             ws = _WORKSPACES[kind, dev, stream] = (t.data_ptr(), t.numel(), t)
     return ws

@@ -36,6 +36,7 @@ def test_graphs_and_eager_calls_share_no_scratch(scratch):
     scratch["id"] = 12                     # another graph on the same stream
     assert paged._held("attn", 0, 5) is paged._NO_WORKSPACE
     assert get(1000)[0] not in (first[0], larger[0], eager[0])
+    assert list(paged._GRAPH_WORKSPACES) == [("attn", 0, 5)]  # an earlier graph's are not held on to
     scratch["id"] = 0
     assert get(1000) is eager
 
