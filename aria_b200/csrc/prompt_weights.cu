@@ -127,6 +127,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -136,13 +141,13 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // 2^x of two values on the multiply-add pipe: x = n + f with n an integer and |f| <= 1/2
 // (n from the low bits of x + 1.5 2^23), a polynomial in f of degree 5 whose coefficients
 // minimise the largest relative error on that interval (Lawson's iteration; 2.3e-7
-// evaluated in f32), and n added to the exponent.  x below -126 gives 0 (-inf does, for
-// masked queries), x above 127 gives 2^127.  NaN stays NaN: it goes round the addition to
-// the exponent, which would make a large finite number of its bits.
+// evaluated in f32), times 2^n.  x below -126 gives 0 (-inf does, for masked queries), x
+// from 127.5 on inf.  NaN stays NaN because 2^n is a factor: added to the exponent, n made
+// a large finite number of the NaN's bits.
 __device__ __forceinline__ uint64_t both(float x) { return pack2(__float_as_uint(x), __float_as_uint(x)); }
 __device__ __forceinline__ void exp2_poly2(float& x, float& y) {
-  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(127.0f));
-  asm("min.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(127.0f));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(128.0f));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(128.0f));
   const uint64_t v = pack2(__float_as_uint(x), __float_as_uint(y));
   const uint64_t t = add2(v, both(12582912.0f));
   const uint64_t f = fma2(add2(t, both(-12582912.0f)), both(-1.0f), v);
@@ -152,13 +157,10 @@ __device__ __forceinline__ void exp2_poly2(float& x, float& y) {
   p = fma2(p, f, both(6.9314694e-1f));
   p = fma2(p, f, both(1.0000001f));
   float p0, p1, t0, t1;
-  unpack2(p, p0, p1);
   unpack2(t, t0, t1);
-  float x0, y0;  // 0, or the NaN
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(x), "f"(0.0f));
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y0) : "f"(y), "f"(0.0f));
-  x = x >= -126.0f ? __int_as_float(__float_as_int(p0) + (__float_as_int(t0) << 23)) : x0;
-  y = y >= -126.0f ? __int_as_float(__float_as_int(p1) + (__float_as_int(t1) << 23)) : y0;
+  unpack2(mul2(p, pack2((__float_as_uint(t0) << 23) + 0x3f800000u, (__float_as_uint(t1) << 23) + 0x3f800000u)), p0, p1);
+  x = x < -126.0f ? 0.0f : p0;
+  y = y < -126.0f ? 0.0f : p1;
 }
 
 // The terms of one block of queries, each taken by selection: those from cmin on that saw
@@ -493,41 +495,46 @@ __global__ void __launch_bounds__(kPwThreads, 1)
     }
   } else if (warp == 2 + kPwSumWarps) {
     // ------------------------------------------------------------ lse rows
-    // (a block's rows are fetched while the one before it waits for its buffer)
+    // (a block's rows are fetched while the one before it waits for its buffer; which rows
+    // they are is worked out one block earlier still)
     int t = blockIdx.x, j = 0, h = 0, qb = 0;
     PromptItem im;
-    auto begin = [&]() {  // the first block of item t, or of the first one after it that has any
+    const float* row = nullptr;  // of block j
+    auto begin = [&]() {         // the first block of item t, or of the first one after it that has any
       for (; t < n_items; t += gridDim.x) {
         im = prompt_item(a, t, n_items);
         if (im.lo < im.hi) {
           j = im.lo;
           h = im.lo / im.nq;
           qb = im.lo - h * im.nq;
+          row = a.lse + ((size_t)im.seq * a.Hkv * a.G + im.hk * a.G + h) * a.T;
           return;
         }
+      }
+    };
+    auto advance = [&]() {
+      if (t >= n_items) return;
+      if (++j == im.hi) {
+        t += gridDim.x;
+        begin();
+      } else if (++qb == im.nq) {
+        qb = 0;
+        row += a.T;
       }
     };
     float next[4];
     auto fetch = [&]() {
       if (t >= n_items) return;
-      const float* row = a.lse + ((size_t)im.seq * a.Hkv * a.G + im.hk * a.G + h) * a.T;
 #pragma unroll
       for (int u = 0; u < 4; u++) {
         const int q = (im.q0 + qb) * kPwB + 32 * u + lane;
         next[u] = q < a.T && q >= a.first ? row[q] : INFINITY;
       }
-      if (++qb == im.nq) {
-        qb = 0;
-        h++;
-      }
-      if (++j == im.hi) {
-        t += gridDim.x;
-        begin();
-      }
     };
     begin();
     bool more = t < n_items;
     fetch();
+    advance();
     for (int g = 0; more; g++) {
       const int b = g % kPwS;
       float v[4];
@@ -553,6 +560,7 @@ __global__ void __launch_bounds__(kPwThreads, 1)
       if (lane == 0) lse_gaps[b] = gap;
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&s_full[b]);
+      advance();
     }
   }
 

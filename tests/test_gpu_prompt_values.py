@@ -45,3 +45,19 @@ def test_rows_that_saw_nothing_give_nothing_whatever_they_hold(value, dh):
     q[0, hidden, 1, 11] = float(value)
     got = _f64(prompt_weights(q, k, torch.from_numpy(rows)[None].float().cuda())[0])
     assert np.all(np.abs(got - ref) <= 5e-5 * ref + 1e-6)
+
+
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("residue", range(16))
+def test_terms_past_the_range_of_f32_are_infinite(residue, dh):
+    """An lse far below the scores, at every position of 16 queries: exp(100) is no f32."""
+    from aria_b200.paged import prompt_weights
+    T, t = 400, 256 + residue
+    q, k = (torch.zeros(1, T, 1, dh, device="cuda").half() for _ in range(2))
+    lse = torch.full((1, 1, T), 100.0, device="cuda")
+    lse[0, 0, t] = -100.0
+    got = prompt_weights(q, k, lse)[0, 0]
+    assert bool(torch.isinf(got[:t + 1]).all()) and bool((got[t + 1:] < 1e-40).all())
+    lse[0, 0, t] = -80.0  # exp(80) is one
+    got = prompt_weights(q, k, lse)[0, 0, :t + 1].double().cpu().numpy()
+    assert np.all(np.abs(got / np.exp(80.0) - 1) <= 3e-5)
