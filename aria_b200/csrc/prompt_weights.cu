@@ -331,11 +331,11 @@ __global__ void __launch_bounds__(kPwThreads, 1)
         }
         it++;
       }
-      if (!ok) {
-        // no MMA of this thread may still write tensor memory when it is freed
-        tc::umma_commit(mma_drain);
-        tc::mbar_wait(mma_drain, 0);
-      }
+      // no MMA of this thread may still write tensor memory when it is freed, nor arrive at a
+      // barrier of a CTA that has left.  (The sums wait for every product, but a warp that gives
+      // up after the last one was issued takes the others along.)
+      tc::umma_commit(mma_drain);
+      tc::mbar_wait(mma_drain, 0);
     }
   } else if (warp < 2 + kPwSumWarps) {
     // ------------------------------------------------------------ sums
