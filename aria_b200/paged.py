@@ -22,7 +22,7 @@ import torch
 from . import _lib
 from ._lib import BF16, F16, PagedKVStruct, call, fastcall
 
-__all__ = ["PagedKV", "attention_paged", "prompt_weights", "evict"]
+__all__ = ["PagedKV", "attention_paged", "prompt_weights", "evict", "clear_workspaces"]
 
 _DTYPES = {torch.float16: F16, torch.bfloat16: BF16}
 # (operator, device, stream) -> (pointer, bytes, tensor): scratch of eager calls, and of the
@@ -74,6 +74,14 @@ def _workspace(kind: str, nbytes: int, dev: int, stream: int, cleared: str = "co
         else:
             ws = _WORKSPACES[kind, dev, stream] = (t.data_ptr(), t.numel(), t)
     return ws
+
+
+def clear_workspaces() -> None:
+    """Forget the scratch of the serving operators; their next calls start from new.  For use
+    after a call during which a wait on the device expired (aria_q4_take_device_error() !=
+    0): it may have left counters behind.  (A graph's scratch is cleared by the graph.)"""
+    _WORKSPACES.clear()
+    _GRAPH_WORKSPACES.clear()
 
 
 def _want(t: torch.Tensor, name: str, dtype, shape, dev: int) -> int:

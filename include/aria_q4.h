@@ -285,7 +285,8 @@ ARIA_Q4_API int aria_attention_prefill(const uint16_t* qkv, int B, int T, int d,
  * an entry outside [0, num_pages) has no page, and its slots are absent: not read,
  * not written, weight 0.  Element strides (multiples of 8) place slot s of page p
  * of head h at p page_stride + s slot_stride + h head_stride, for K and V alike.
- * A contiguous cache [M][max_seq][d] is one whose pages lie in order.  head_dim
+ * A contiguous cache [M][max_seq][d] is one whose pages lie in order.  Sequences may
+ * share pages as long as neither appends to them nor is evicted from.  head_dim
  * 32, 64, 128 or 256; pages 16-byte aligned; M <= 4096. */
 typedef struct {
   void* k_pages;            /* f16 or bf16 (dtype) */

@@ -92,3 +92,22 @@ def test_counts_past_32_bits_are_refused(n):
     for out in (None, torch.zeros(1, 2, 8, device="cuda")):
         with pytest.raises(ValueError):
             prompt_weights(x, x, lse, out=out, first_query=n)
+
+
+def test_counters_left_behind_are_cleared_with_the_scratch():
+    """Counters as an expired wait would leave them (set by hand): the sums of a cut call are wrong
+    until the scratch is cleared, and right after."""
+    from aria_b200 import paged
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, k = (torch.randn(1, 4096, 1, 64, generator=g, device="cuda").half() for _ in range(2))
+    lse = torch.full((1, 1, 4096), 9.0, device="cuda")
+    want = paged.prompt_weights(q, k, lse).clone()
+    held = [w for (kind, _, _), w in paged._WORKSPACES.items() if kind == "prompt"]
+    assert any(w[1] > 64 * 512 for w in held)  # the call is cut: it joins parts
+    for w in held:
+        w[2][:4096].view(torch.int32).fill_(1)
+        w[2][4096:].zero_()  # (the parts of the call before this one)
+    bad = paged.prompt_weights(q, k, lse).clone()
+    paged.clear_workspaces()
+    assert not paged._WORKSPACES
+    assert torch.equal(paged.prompt_weights(q, k, lse), want) and not torch.equal(bad, want)
