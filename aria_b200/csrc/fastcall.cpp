@@ -4,7 +4,7 @@
 // One token's kernels run for 5 to 10 microseconds; checking a dozen tensors and
 // converting two dozen arguments through ctypes takes the host as long again.  Here the
 // checks of aria_b200/paged.py and logits.py are made in C++ and the C ABI is called
-// directly (attention of one sequence: 4.7 us of host time per call instead of 11.9,
+// directly (attention of one sequence: 4.8 us of host time per call instead of 11.9,
 // most of it the launch and the lse's allocation; logits of one row: 6.5 instead of 16).
 // A function returns None when anything is unusual and nothing was launched -- an argument
 // that does not pass, a workspace that has to grow, a call that the library refuses -- and

@@ -13,10 +13,12 @@
 // its row of S in registers: no reduction across threads, nothing but the finished
 // sums leaves the SM.  Per 128 x 128 block: 2 dh / 128 MMA cycles x 128 (256 at
 // dh = 64) against 16384 exponentials at 16 a cycle (1024 cycles), so the exponential
-// unit is the bound: it is 84% busy at 2 x 8190 x 32 heads of 128 (597 us at the 1.7 GHz
-// that the power limit leaves).  At dh = 64 one pair in eight goes through a polynomial
-// on the multiply-add pipe instead (558 -> 520 us at that size; two pairs: 531); at 128
-// the added instructions lower the clock by more than they save (597 -> 619).
+// unit is the bound: it is 85% busy over 2 x 8190 positions x 32 heads of 128 (8 groups of
+// 4, queries from 2047 on: 596 us, 680 to 690 once the power limit holds the clock at 1.5
+// to 1.7 GHz), 65% over 4 x 2048 x 14 heads of 64, where the start and the items' ends
+// count.  At dh = 64 one pair in eight goes through a polynomial on the multiply-add pipe
+// instead (the longer size with heads of 64: 558 -> 520 us; two pairs: 531); at 128 the
+// added instructions lowered the clock by more than they saved (597 -> 619).
 //
 // Persistent, one CTA per SM; an item is (sequence, key/value head, key block) or, where
 // those are few, a part of its query blocks (the last part to finish adds the parts' sums
@@ -26,8 +28,9 @@
 //   warps 2-17  sums: a warp per TMEM lane quadrant and S buffer, so that the four
 //               warps of a sub-partition are at different blocks and keep its
 //               exponential unit busy through one another's waits.  (Four warps per
-//               block, a quarter of the queries each: 55 us at 4 x 2048 x 14 heads;
-//               two warps: 70 us, the unit 40% busy; so: 41 us.)
+//               block, a quarter of the queries each: 55 us at 4 x 2048 x 14 heads,
+//               the same call repeated; two warps: 70 us, the unit 40% busy; so: 41 us,
+//               44 with other inputs each time.)
 //   warp 18     lse rows of the query blocks -> shared memory, negated, in the log2 domain;
 //               -inf for queries before `first` or past the end, whose terms vanish, and
 //               for those whose lse is -inf, with a word by which the block's scores are
@@ -618,8 +621,8 @@ static cudaError_t launch_prompt_t(const PromptArgs& a, const CUtensorMap& tq, c
 // Parts that a key block's sums are cut into.  A part costs about as much as 4 blocks
 // (its K block, an empty pipeline, the join), so sums stay whole unless the longest is
 // more than twice an SM's share of all blocks, or 16: then the parts are one and a half
-// such shares.  (One head of 8192 positions, 64 key blocks of 64 to 1: 43 us uncut, 22
-// us cut; 14 heads of 2048, 16 blocks at most: 17 us uncut, 26 cut in two.)
+// such shares.  (One head of 8192 positions, 64 key blocks of 64 to 1: 43 us uncut, 21
+// to 25 cut; 14 heads of 2048, 16 blocks at most: 17 us uncut, 26 cut in two.)
 constexpr int kPwMaxCut = 1024;  // key blocks that may be cut: a fixed number of counters
 static int prompt_splits(int B, int T, int Hkv, int G, int first) {
   const long long n_kt = (T + kPwB - 1) / kPwB, base = n_kt * B * Hkv;
